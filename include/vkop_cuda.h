@@ -198,6 +198,152 @@ int vkop_cuda_softmax_topk_merge(const vkop_softmax_topk_desc *desc, const void 
 int vkop_cuda_sample_topk(const void *values, int32_t dtype, const void *indices, int32_t index_dtype, int64_t rows,
                           int32_t k, float top_p, const float *u, int32_t *out_choice, void *out_token, void *stream);
 
+/* ------------------------------------------------------------------------ */
+/* A speculative decoding step (no counterpart in the reference): several
+ * drafted tokens a sequence are scored by the model at once, the ones that a
+ * verification against the target's probabilities accepts are kept.
+ *
+ * The drafted tokens of a sequence form a tree of `nodes` nodes.  Node 0 is
+ * the last token already decided, nodes 1.. are drafted, parents[b][i] < i is
+ * the node that node i continues (parents == NULL: a chain, i continues
+ * i - 1); parents[b][0] is not read.  A node whose parent is not in [0, i) is
+ * the child of nobody and has no ancestors.  num_nodes[b] in [0, nodes] nodes
+ * of sequence b are in use (NULL: all; larger values count as `nodes`,
+ * negative ones as 0), the others are padding.  The key and value of node i
+ * lie in the cache at position context[b] + i.
+ *
+ * Verification of drafted tokens against the target's probabilities from
+ * given random numbers.  target [batch, nodes, vocab]: row n holds the
+ * target's probabilities of the token after node n; draft
+ * [batch, draft_rows, vocab]: row n the distribution that the children of
+ * node n were drawn from (independently of one another), as
+ * vkop_cuda_softmax writes them.  Children of a node >= draft_rows, and all
+ * when draft_rows is 0, count as drafted with certainty.
+ *
+ * The walk starts at node 0 and tests the children of the node it stands on
+ * in ascending order.  Of a node's distribution p (and the draft's q) what is
+ * left after some rejections is max(p - c q, 0) with mass D; c = 0, D = 1 at
+ * first.  Child i with token t is accepted when
+ *     u[b][i] * D * q(t) < max(p(t) - c q(t), 0),
+ * and the walk goes on from it; a rejection adds D to c and makes D the sum
+ * of max(p - c q, 0) over the vocabulary.  With certain drafts child i is
+ * accepted when u[b][i] * D < p(t); a rejection takes p(t) out of D and out
+ * of p.  The last token is drawn from what is left at the last node: the
+ * first index whose prefix sum exceeds u[b][0] times the whole sum (where
+ * nothing is left: from p; where p is all zero: -1).  For independent uniform
+ * numbers the tokens have the target's distribution.  All of it is computed
+ * in 64 bits.  Entries that are negative, NaN or infinite count as zero; a
+ * child whose token is not in [0, vocab) is passed over.
+ *
+ * u [batch, nodes] uniform numbers in [0, 1).  out_path [batch, nodes]: the
+ * accepted nodes in order, node 0 first, then -1; out_count [batch]: how many
+ * (0 where num_nodes is 0); out_token [batch]: the last token, -1 for an
+ * empty sequence; out_chance [batch, nodes] (may be NULL): the probability
+ * with which a tested node was accepted, min(1, left / (D q)), else 0.
+ * Strides are in elements, rows of the vocabulary are contiguous; 0 means
+ * dense. */
+typedef struct vkop_draft_verify_desc {
+    int64_t batch;
+    int64_t vocab;               /* 1 .. 2^31 - 1 */
+    int64_t target_batch_stride;
+    int64_t target_node_stride;
+    int64_t draft_batch_stride;
+    int64_t draft_node_stride;
+    int32_t nodes;               /* 1 .. 1024 */
+    int32_t draft_rows;          /* 0 .. nodes */
+    int32_t dtype;               /* vkop_dtype of target and draft */
+    int32_t index_dtype;         /* vkop_index_dtype of tokens and out_token */
+} vkop_draft_verify_desc;
+
+int vkop_cuda_draft_verify(const vkop_draft_verify_desc *desc, const void *target, const void *draft,
+                           const void *tokens, const int32_t *parents, const int32_t *num_nodes, const float *u,
+                           int32_t *out_path, int32_t *out_count, void *out_token, float *out_chance, void *stream);
+
+/* Attention of a tree of drafted tokens over a paged cache.  Node i of
+ * sequence b attends the context, positions [0, context[b]), and of the
+ * drafted positions its ancestors' and its own.  nodes = 1 is the plain
+ * attention of one new token.
+ *
+ * q, out [batch, nodes, q_heads, head_dim]; query head h reads cache head
+ * h / (q_heads / kv_heads).  k_cache, v_cache [num_pages, page_size,
+ * kv_heads, head_dim] by strides (a [num_pages, kv_heads, page_size,
+ * head_dim] cache has other page / token / head strides); position p of
+ * sequence b lies in page page_table[b][p / page_size], slot p % page_size.
+ * Entries behind a sequence's last position are not read; a position whose
+ * page is not in [0, num_pages), or that lies behind the table, is left out.
+ * A negative context counts as 0.
+ *
+ *     out = softmax(scale * q k^T over the attended positions) v
+ *
+ * with scores, sums and accumulators in 32 bits; 16-bit inputs multiply as
+ * such, weights rounded to the inputs' type.  out_lse [batch, nodes, q_heads]
+ * (may be NULL): the natural logarithm of the sum of exp(score).  A row that
+ * attends nothing, a padding node's among them, is written as zeros with
+ * lse = -inf.  Values of positions that a row does not attend never reach it,
+ * whatever they hold.
+ *
+ * max_context: no context[b] is larger as far as the caller knows (it sizes
+ * the launch and the scratch; a longer context is still attended in full,
+ * only slower); 0 means max_pages * page_size.  Workspace: scratch only,
+ * 16-byte aligned, needs no clearing and keeps nothing between calls.
+ * Strides are in elements, head_dim is contiguous; 0 means dense. */
+typedef struct vkop_tree_attention_desc {
+    int64_t batch;
+    int64_t num_pages;
+    int64_t max_context;
+    int64_t q_batch_stride, q_node_stride, q_head_stride;
+    int64_t out_batch_stride, out_node_stride, out_head_stride;
+    int64_t k_page_stride, k_token_stride, k_head_stride;
+    int64_t v_page_stride, v_token_stride, v_head_stride;
+    int64_t table_stride;        /* elements between rows of page_table; 0 means max_pages */
+    int32_t nodes;               /* 1 .. 128 */
+    int32_t q_heads;             /* a multiple of kv_heads */
+    int32_t kv_heads;
+    int32_t head_dim;            /* a multiple of 8, at most 256 */
+    int32_t page_size;           /* 1 .. 65536 */
+    int32_t max_pages;           /* columns of page_table */
+    int32_t dtype;               /* vkop_dtype of q, the caches and out */
+    float scale;                 /* finite */
+} vkop_tree_attention_desc;
+
+int vkop_cuda_tree_attention_workspace(const vkop_tree_attention_desc *desc, size_t *bytes);
+int vkop_cuda_tree_attention(const vkop_tree_attention_desc *desc, const void *q, const void *k_cache,
+                             const void *v_cache, const int32_t *page_table, const int32_t *context,
+                             const int32_t *parents, const int32_t *num_nodes, void *out, float *out_lse,
+                             void *workspace, size_t workspace_bytes, void *stream);
+
+/* Keeps the accepted path's rows of a paged cache: in every layer, the row at
+ * position context[b] + path[b][i] moves to position context[b] + i, for
+ * 0 < i < count[b] (path and count as vkop_cuda_draft_verify writes them), and
+ * out_context[b] = context[b] + count[b].  In place; rows that are not moved
+ * keep their values.  A path that is not ascending or leaves [0, nodes) ends
+ * there, and out_context counts up to it; a row whose page (source or target)
+ * is not in [0, num_pages) or lies behind the table stays where it is.
+ *
+ * k_cache, v_cache [layers, num_pages, page_size, kv_heads, head_dim] by
+ * strides, as above; v_cache may be NULL (one cache only).  The pages from
+ * position context[b] on belong to sequence b alone.  out_context does not
+ * overlap context. */
+typedef struct vkop_cache_compact_desc {
+    int64_t batch;
+    int64_t num_pages;
+    int64_t k_layer_stride, k_page_stride, k_token_stride, k_head_stride;
+    int64_t v_layer_stride, v_page_stride, v_token_stride, v_head_stride;
+    int64_t table_stride;
+    int32_t layers;              /* 0 .. 65535 */
+    int32_t nodes;               /* columns of path, 1 .. 1024 */
+    int32_t kv_heads;
+    int32_t head_dim;
+    int32_t page_size;
+    int32_t max_pages;
+    int32_t dtype;
+    int32_t reserved;            /* 0 */
+} vkop_cache_compact_desc;
+
+int vkop_cuda_cache_compact(const vkop_cache_compact_desc *desc, void *k_cache, void *v_cache,
+                            const int32_t *page_table, const int32_t *context, const int32_t *path,
+                            const int32_t *count, int32_t *out_context, void *stream);
+
 /* Packet exchange over peer memory instead of an all-gather (no counterpart in
  * the reference, which is single-device).  Every rank owns a receive buffer
  * `slots` of 2 * world * packets_bytes bytes and `flags` of 2 * world uint32,

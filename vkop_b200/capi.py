@@ -29,6 +29,7 @@ EXPORTS = [
     "vkop_cuda_static_scratch_bytes", "vkop_cuda_softmax_topk_static",
     "vkop_cuda_packets_push", "vkop_cuda_packets_wait", "vkop_cuda_packets_exchange_all_ranks", "vkop_cuda_yolo_nms",
     "vkop_cuda_sample_topk", "vkop_cuda_topk_axis_workspace", "vkop_cuda_topk_axis",
+    "vkop_cuda_draft_verify", "vkop_cuda_tree_attention_workspace", "vkop_cuda_tree_attention", "vkop_cuda_cache_compact",
 ]
 
 
@@ -54,6 +55,32 @@ class NmsDesc(C.Structure):
     _fields_ = [("num_batch", C.c_int32), ("num_class", C.c_int32), ("num_boxes", C.c_int32),
                 ("center_point_box", C.c_int32), ("max_output_boxes_per_class", C.c_int32), ("pre_topk", C.c_int32),
                 ("iou_threshold", C.c_float), ("score_threshold", C.c_float), ("capacity_rows", C.c_int64)]
+
+
+class DraftVerifyDesc(C.Structure):
+    _fields_ = [("batch", C.c_int64), ("vocab", C.c_int64), ("target_batch_stride", C.c_int64),
+                ("target_node_stride", C.c_int64), ("draft_batch_stride", C.c_int64), ("draft_node_stride", C.c_int64),
+                ("nodes", C.c_int32), ("draft_rows", C.c_int32), ("dtype", C.c_int32), ("index_dtype", C.c_int32)]
+
+
+class TreeAttentionDesc(C.Structure):
+    _fields_ = [("batch", C.c_int64), ("num_pages", C.c_int64), ("max_context", C.c_int64),
+                ("q_batch_stride", C.c_int64), ("q_node_stride", C.c_int64), ("q_head_stride", C.c_int64),
+                ("out_batch_stride", C.c_int64), ("out_node_stride", C.c_int64), ("out_head_stride", C.c_int64),
+                ("k_page_stride", C.c_int64), ("k_token_stride", C.c_int64), ("k_head_stride", C.c_int64),
+                ("v_page_stride", C.c_int64), ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64),
+                ("table_stride", C.c_int64), ("nodes", C.c_int32), ("q_heads", C.c_int32), ("kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("page_size", C.c_int32), ("max_pages", C.c_int32), ("dtype", C.c_int32),
+                ("scale", C.c_float)]
+
+
+class CacheCompactDesc(C.Structure):
+    _fields_ = [("batch", C.c_int64), ("num_pages", C.c_int64), ("k_layer_stride", C.c_int64),
+                ("k_page_stride", C.c_int64), ("k_token_stride", C.c_int64), ("k_head_stride", C.c_int64),
+                ("v_layer_stride", C.c_int64), ("v_page_stride", C.c_int64), ("v_token_stride", C.c_int64),
+                ("v_head_stride", C.c_int64), ("table_stride", C.c_int64), ("layers", C.c_int32), ("nodes", C.c_int32),
+                ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("page_size", C.c_int32), ("max_pages", C.c_int32),
+                ("dtype", C.c_int32), ("reserved", C.c_int32)]
 
 
 class VkopError(RuntimeError):
@@ -93,6 +120,10 @@ def lib() -> C.CDLL:
         L.vkop_cuda_packets_exchange_all_ranks.argtypes = [vp, sz, vp, vp, C.c_int32, C.c_uint32, vp, C.c_uint32, vp, vp]
         L.vkop_cuda_yolo_nms.argtypes = [C.POINTER(NmsDesc), vp, vp, vp, vp, sz, vp]
         L.vkop_cuda_sample_topk.argtypes = [vp, C.c_int32, vp, C.c_int32, C.c_int64, C.c_int32, C.c_float, vp, vp, vp, vp]
+        L.vkop_cuda_draft_verify.argtypes = [C.POINTER(DraftVerifyDesc)] + [vp] * 11
+        L.vkop_cuda_tree_attention_workspace.argtypes = [C.POINTER(TreeAttentionDesc), C.POINTER(sz)]
+        L.vkop_cuda_tree_attention.argtypes = [C.POINTER(TreeAttentionDesc)] + [vp] * 10 + [sz, vp]
+        L.vkop_cuda_cache_compact.argtypes = [C.POINTER(CacheCompactDesc)] + [vp] * 8
         L.vkop_cuda_static_scratch_bytes.restype = sz
         L.vkop_cuda_softmax_topk_static.argtypes = [C.POINTER(SoftmaxTopkDesc), vp, vp, vp, vp]
         _lib = L
@@ -245,6 +276,166 @@ def sample_topk(values: torch.Tensor, indices: torch.Tensor, top_p: float, u: to
                                       I64 if indices.dtype == torch.int64 else I32, rows, k, float(top_p), u.data_ptr(),
                                       choice.data_ptr(), token.data_ptr(), _stream()), "sample_topk")
     return choice, token
+
+
+def _one_device(what: str, *tensors) -> torch.device:
+    """The device that all the tensors lie on (None among them is passed over)."""
+    device = tensors[0].device
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device != device):
+            raise RuntimeError(f"{what}: vkop_b200 runs on CUDA device memory only, all tensors on one device")
+    return device
+
+
+def _whole(what: str, name: str, t, shape, dtype=torch.int32):
+    """Checks a small dense argument: its type, its shape and that it is contiguous."""
+    if t is not None and (t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous()):
+        raise ValueError(f"{what}: {name} is a contiguous {dtype} tensor of shape {tuple(shape)}, "
+                         f"got {t.dtype} {tuple(t.shape)}")
+
+
+def _strides(what: str, name: str, t: torch.Tensor, ndim: int):
+    """Strides of the leading dimensions, in elements; the last dimension is contiguous and nothing is broadcast."""
+    if t.dim() != ndim or t.dtype not in _TORCH_DTYPE:
+        raise ValueError(f"{what}: {name} is a float32, float16 or bfloat16 tensor of {ndim} dimensions")
+    strides, shape = t.stride(), t.shape
+    if (strides[-1] != 1 and shape[-1] > 1) or any(s == 0 and n > 1 for s, n in zip(strides, shape)):
+        raise ValueError(f"{what}: {name} has a contiguous last dimension and no broadcast one")
+    return [s if n > 1 else 0 for s, n in zip(strides[:-1], shape[:-1])]
+
+
+def draft_verify(target: torch.Tensor, tokens: torch.Tensor, u: torch.Tensor, draft: torch.Tensor | None = None,
+                 parents: torch.Tensor | None = None, num_nodes: torch.Tensor | None = None, chances: bool = False):
+    """Verifies a tree (parents given) or chain of drafted tokens against the target's probabilities.
+
+    target [batch, nodes, vocab]; tokens int32 or int64 [batch, nodes] (column 0, the last token already decided, is not
+    read); u float32 [batch, nodes] uniform numbers, column 0 for the last token; draft [batch, draft_rows, vocab], the
+    distributions that the children of nodes 0 .. draft_rows - 1 were drawn from, or None for tokens drafted with certainty;
+    parents int32 [batch, nodes]; num_nodes int32 [batch].
+    Returns (path int32 [batch, nodes], count int32 [batch], token [batch]), and chance float32 [batch, nodes] if asked."""
+    what = "draft_verify"
+    device = _one_device(what, target, tokens, u, draft, parents, num_nodes)
+    ts = _strides(what, "target", target, 3)
+    batch, nodes, vocab = target.shape
+    ds, rows = [0, 0], 0
+    if draft is not None:
+        ds, rows = _strides(what, "draft", draft, 3), draft.shape[1]
+        if draft.dtype != target.dtype or draft.shape[0] != batch or draft.shape[2] != vocab:
+            raise ValueError("draft_verify: draft has the type, batch and vocabulary of target")
+    if tokens.dtype not in (torch.int32, torch.int64):
+        raise ValueError("draft_verify: tokens are int32 or int64")
+    _whole(what, "tokens", tokens, (batch, nodes), tokens.dtype)
+    _whole(what, "u", u, (batch, nodes), torch.float32)
+    _whole(what, "parents", parents, (batch, nodes))
+    _whole(what, "num_nodes", num_nodes, (batch,))
+    desc = DraftVerifyDesc(batch, vocab, ts[0], ts[1], ds[0], ds[1], nodes, rows, dtype_tag(target),
+                           I64 if tokens.dtype == torch.int64 else I32)
+    path = torch.empty((batch, nodes), dtype=torch.int32, device=device)
+    count = torch.empty(batch, dtype=torch.int32, device=device)
+    token = torch.empty(batch, dtype=tokens.dtype, device=device)
+    chance = torch.empty((batch, nodes), dtype=torch.float32, device=device) if chances else None
+    with torch.cuda.device(device):
+        check(lib().vkop_cuda_draft_verify(C.byref(desc), target.data_ptr(), _ptr(draft), tokens.data_ptr(), _ptr(parents),
+                                           _ptr(num_nodes), u.data_ptr(), path.data_ptr(), count.data_ptr(),
+                                           token.data_ptr(), _ptr(chance), _stream()), what)
+    return (path, count, token, chance) if chances else (path, count, token)
+
+
+def _tree_attention_desc(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                         scale: float | None, max_context: int, out: torch.Tensor | None) -> TreeAttentionDesc:
+    what = "tree_attention"
+    qs, ks, vs = _strides(what, "q", q, 4), _strides(what, "k_cache", k_cache, 4), _strides(what, "v_cache", v_cache, 4)
+    os_ = _strides(what, "out", out, 4) if out is not None else [0, 0, 0]
+    batch, nodes, heads, dim = q.shape
+    pages, page_size, kv_heads, kv_dim = k_cache.shape
+    if k_cache.shape != v_cache.shape or kv_dim != dim or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise ValueError("tree_attention: k_cache and v_cache are [pages, page_size, kv_heads, head_dim] of q's type and head_dim")
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch or \
+            (page_table.shape[1] > 1 and page_table.stride(1) != 1) or (batch > 1 and page_table.stride(0) < page_table.shape[1]):
+        raise ValueError("tree_attention: page_table is int32 [batch, max_pages]")
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype):
+        raise ValueError("tree_attention: out has the shape and type of q")
+    return TreeAttentionDesc(batch, pages, max_context, *qs, *os_, *ks, *vs, page_table.stride(0) if batch > 1 else 0, nodes,
+                             heads, kv_heads, dim, page_size, page_table.shape[1], dtype_tag(q),
+                             dim ** -0.5 if scale is None else scale)
+
+
+def tree_attention_workspace_bytes(q, k_cache, v_cache, page_table, max_context: int = 0) -> int:
+    """Scratch that tree_attention needs for tensors of these shapes."""
+    n = C.c_size_t(0)
+    desc = _tree_attention_desc(q, k_cache, v_cache, page_table, None, max_context, None)
+    check(lib().vkop_cuda_tree_attention_workspace(C.byref(desc), C.byref(n)), "tree_attention_workspace")
+    return int(n.value)
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                   context: torch.Tensor, parents: torch.Tensor | None = None, num_nodes: torch.Tensor | None = None,
+                   scale: float | None = None, max_context: int = 0, return_lse: bool = False,
+                   workspace: torch.Tensor | None = None, out: torch.Tensor | None = None):
+    """Attention of the nodes of a token tree (parents None: a chain) over a paged cache that holds the context and, from
+    position context[b] on, the nodes themselves.
+
+    q [batch, nodes, q_heads, head_dim]; k_cache, v_cache [pages, page_size, kv_heads, head_dim], any strides with a
+    contiguous last dimension; page_table int32 [batch, max_pages]; context, num_nodes int32 [batch]; parents int32
+    [batch, nodes]; max_context: an upper bound of context that the caller knows (0: the table's width).  workspace: a
+    uint8 tensor of tree_attention_workspace_bytes() to use instead of torch's allocator.
+    Returns out like q, and lse float32 [batch, nodes, q_heads] if asked."""
+    what = "tree_attention"
+    device = _one_device(what, q, k_cache, v_cache, page_table, context, parents, num_nodes, workspace, out)
+    desc = _tree_attention_desc(q, k_cache, v_cache, page_table, scale, max_context, out)
+    batch, nodes, heads = desc.batch, desc.nodes, desc.q_heads
+    _whole(what, "context", context, (batch,))
+    _whole(what, "parents", parents, (batch, nodes))
+    _whole(what, "num_nodes", num_nodes, (batch,))
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    lse = torch.empty((batch, nodes, heads), dtype=torch.float32, device=device) if return_lse else None
+    L = lib()
+    with torch.cuda.device(device):
+        if workspace is None:
+            need = C.c_size_t(0)
+            check(L.vkop_cuda_tree_attention_workspace(C.byref(desc), C.byref(need)), what)
+            if need.value:
+                workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
+        nbytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+        check(L.vkop_cuda_tree_attention(C.byref(desc), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                                         page_table.data_ptr(), context.data_ptr(), _ptr(parents), _ptr(num_nodes),
+                                         out.data_ptr(), _ptr(lse), _ptr(workspace), nbytes, _stream()), what)
+    return (out, lse) if return_lse else out
+
+
+def cache_compact(k_cache: torch.Tensor, v_cache: torch.Tensor | None, page_table: torch.Tensor, context: torch.Tensor,
+                  path: torch.Tensor, count: torch.Tensor) -> torch.Tensor:
+    """Moves the cache rows of an accepted path (as draft_verify returns it) to the front of the drafted positions, in
+    place.  k_cache, v_cache [layers, pages, page_size, kv_heads, head_dim], or without the first dimension for one layer.
+    Returns the new context lengths, int32 [batch]."""
+    what = "cache_compact"
+    device = _one_device(what, k_cache, v_cache, page_table, context, path, count)
+    if k_cache.dim() == 4:
+        k_cache, v_cache = k_cache[None], v_cache[None] if v_cache is not None else None
+    ks = _strides(what, "k_cache", k_cache, 5)
+    vs = _strides(what, "v_cache", v_cache, 5) if v_cache is not None else [0] * 4
+    if v_cache is not None and (v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype):
+        raise ValueError("cache_compact: k_cache and v_cache have one shape and type")
+    layers, pages, page_size, heads, dim = k_cache.shape
+    batch = context.shape[0]
+    if path.dim() != 2:
+        raise ValueError("cache_compact: path is int32 [batch, nodes]")
+    nodes = path.shape[1]
+    _whole(what, "context", context, (batch,))
+    _whole(what, "path", path, (batch, nodes))
+    _whole(what, "count", count, (batch,))
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch or \
+            (page_table.shape[1] > 1 and page_table.stride(1) != 1) or (batch > 1 and page_table.stride(0) < page_table.shape[1]):
+        raise ValueError("cache_compact: page_table is int32 [batch, max_pages]")
+    desc = CacheCompactDesc(batch, pages, *ks, *vs, page_table.stride(0) if batch > 1 else 0, layers, nodes, heads, dim,
+                            page_size, page_table.shape[1], dtype_tag(k_cache), 0)
+    lengths = torch.empty(batch, dtype=torch.int32, device=device)
+    with torch.cuda.device(device):
+        check(lib().vkop_cuda_cache_compact(C.byref(desc), k_cache.data_ptr(), _ptr(v_cache), page_table.data_ptr(),
+                                            context.data_ptr(), path.data_ptr(), count.data_ptr(), lengths.data_ptr(),
+                                            _stream()), what)
+    return lengths
 
 
 def packets_push(packets: torch.Tensor, peer_slots: torch.Tensor, peer_flags: torch.Tensor, rank: int, world: int,

@@ -381,6 +381,128 @@ int vkop_cuda_sample_topk(const void *values, int32_t dtype, const void *indices
                               static_cast<cudaStream_t>(stream));
 }
 
+static bool float_dtype(int32_t t) { return t == VKOP_F32 || t == VKOP_F16 || t == VKOP_BF16; }
+static bool misaligned(const void *p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
+static size_t element_bytes(int32_t dtype) { return dtype == VKOP_F32 ? 4 : 2; }
+
+int vkop_cuda_draft_verify(const vkop_draft_verify_desc *desc, const void *target, const void *draft,
+                           const void *tokens, const int32_t *parents, const int32_t *num_nodes, const float *u,
+                           int32_t *out_path, int32_t *out_count, void *out_token, float *out_chance, void *stream) {
+    if (!desc)
+        return VKOP_INVALID_ARG;
+    const vkop_draft_verify_desc &d = *desc;
+    if (d.batch < 0 || d.batch > (1 << 24) || d.vocab < 1 || d.vocab > 0x7FFFFFFFll || d.nodes < 1 || d.nodes > 1024 ||
+        d.draft_rows < 0 || d.draft_rows > d.nodes || !float_dtype(d.dtype) ||
+        (d.index_dtype != VKOP_I32 && d.index_dtype != VKOP_I64))
+        return VKOP_INVALID_ARG;
+    if (d.target_node_stride < 0 || d.target_batch_stride < 0 || d.draft_node_stride < 0 || d.draft_batch_stride < 0 ||
+        (d.target_node_stride != 0 && d.target_node_stride < d.vocab && d.nodes > 1) ||
+        (d.draft_node_stride != 0 && d.draft_node_stride < d.vocab && d.draft_rows > 1))
+        return VKOP_INVALID_ARG;
+    if (d.batch == 0)
+        return VKOP_OK;
+    if (!target || (d.draft_rows > 0 && !draft) || !tokens || !u || !out_path || !out_count || !out_token)
+        return VKOP_INVALID_ARG;
+    const size_t esz = element_bytes(d.dtype), isz = d.index_dtype == VKOP_I64 ? 8 : 4;
+    if (misaligned(target, esz) || misaligned(draft, esz) || misaligned(tokens, isz) || misaligned(out_token, isz) ||
+        misaligned(parents, 4) || misaligned(num_nodes, 4) || misaligned(u, 4) || misaligned(out_path, 4) ||
+        misaligned(out_count, 4) || misaligned(out_chance, 4))
+        return VKOP_INVALID_ARG;
+    return launch_draft_verify(d, target, draft, tokens, parents, num_nodes, u, out_path, out_count, out_token, out_chance,
+                               static_cast<cudaStream_t>(stream));
+}
+
+static int validate_tree_attention(const vkop_tree_attention_desc *desc) {
+    if (!desc)
+        return VKOP_INVALID_ARG;
+    const vkop_tree_attention_desc &d = *desc;
+    if (d.batch < 0 || d.batch > 65535 || d.num_pages < 0 || d.num_pages > 0x7FFFFFFFll || d.max_context < 0 ||
+        d.max_context > 0x7FFFFFFFll - 65536 || d.nodes < 1 || d.nodes > 128 || d.kv_heads < 1 || d.kv_heads > 1024 ||
+        d.q_heads < d.kv_heads || d.q_heads % d.kv_heads != 0 || d.q_heads / d.kv_heads > 256 || d.head_dim < 8 || d.head_dim > 256 ||
+        d.head_dim % 8 != 0 || d.page_size < 1 || d.page_size > 65536 || d.max_pages < 0 || !float_dtype(d.dtype) ||
+        !std::isfinite(d.scale))
+        return VKOP_INVALID_ARG;
+    if (static_cast<int64_t>(d.max_pages) * d.page_size > 0x7FFFFFFFll - 65536)
+        return VKOP_UNSUPPORTED;
+    if (static_cast<int64_t>(d.nodes) * (d.q_heads / d.kv_heads) / 8 * d.kv_heads > 60000)
+        return VKOP_UNSUPPORTED;
+    for (int64_t s : {d.q_batch_stride, d.q_node_stride, d.q_head_stride, d.out_batch_stride, d.out_node_stride, d.out_head_stride,
+                      d.k_page_stride, d.k_token_stride, d.k_head_stride, d.v_page_stride, d.v_token_stride, d.v_head_stride,
+                      d.table_stride})
+        if (s < 0)
+            return VKOP_INVALID_ARG;
+    if (d.table_stride != 0 && d.table_stride < d.max_pages && d.batch > 1)
+        return VKOP_INVALID_ARG;
+    return VKOP_OK;
+}
+
+int vkop_cuda_tree_attention_workspace(const vkop_tree_attention_desc *desc, size_t *bytes) {
+    const int rc = validate_tree_attention(desc);
+    if (rc != VKOP_OK)
+        return rc;
+    if (!bytes)
+        return VKOP_INVALID_ARG;
+    return plan_tree_attention(*desc, bytes);
+}
+
+int vkop_cuda_tree_attention(const vkop_tree_attention_desc *desc, const void *q, const void *k_cache,
+                             const void *v_cache, const int32_t *page_table, const int32_t *context,
+                             const int32_t *parents, const int32_t *num_nodes, void *out, float *out_lse,
+                             void *workspace, size_t workspace_bytes, void *stream) {
+    int rc = validate_tree_attention(desc);
+    if (rc != VKOP_OK || desc->batch == 0)
+        return rc;
+    const bool cache = desc->num_pages > 0 && desc->max_pages > 0;
+    if (!q || !context || !out || (cache && (!k_cache || !v_cache || !page_table)))
+        return VKOP_INVALID_ARG;
+    const size_t esz = element_bytes(desc->dtype);
+    if (misaligned(q, esz) || misaligned(k_cache, esz) || misaligned(v_cache, esz) || misaligned(out, esz) ||
+        misaligned(page_table, 4) || misaligned(context, 4) || misaligned(parents, 4) || misaligned(num_nodes, 4) ||
+        misaligned(out_lse, 4))
+        return VKOP_INVALID_ARG;
+    size_t need = 0;
+    rc = plan_tree_attention(*desc, &need);
+    if (rc != VKOP_OK)
+        return rc;
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        return VKOP_WORKSPACE_TOO_SMALL;
+    if (need > 0 && misaligned(workspace, 16))
+        return VKOP_INVALID_ARG;
+    return launch_tree_attention(*desc, q, k_cache, v_cache, page_table, context, parents, num_nodes, out, out_lse, workspace,
+                                 static_cast<cudaStream_t>(stream));
+}
+
+int vkop_cuda_cache_compact(const vkop_cache_compact_desc *desc, void *k_cache, void *v_cache,
+                            const int32_t *page_table, const int32_t *context, const int32_t *path,
+                            const int32_t *count, int32_t *out_context, void *stream) {
+    if (!desc)
+        return VKOP_INVALID_ARG;
+    const vkop_cache_compact_desc &d = *desc;
+    if (d.batch < 0 || d.batch > (1 << 24) || d.num_pages < 0 || d.num_pages > 0x7FFFFFFFll || d.layers < 0 || d.layers > 32767 ||
+        d.nodes < 1 || d.nodes > 1024 || d.kv_heads < 1 || d.kv_heads > 65536 || d.head_dim < 1 || d.head_dim > 65536 ||
+        d.page_size < 1 || d.page_size > 65536 || d.max_pages < 0 || !float_dtype(d.dtype) || d.reserved != 0)
+        return VKOP_INVALID_ARG;
+    for (int64_t s : {d.k_layer_stride, d.k_page_stride, d.k_token_stride, d.k_head_stride, d.v_layer_stride, d.v_page_stride,
+                      d.v_token_stride, d.v_head_stride, d.table_stride})
+        if (s < 0)
+            return VKOP_INVALID_ARG;
+    if (d.table_stride != 0 && d.table_stride < d.max_pages && d.batch > 1)
+        return VKOP_INVALID_ARG;
+    if (d.batch == 0)
+        return VKOP_OK;
+    const bool cache = d.layers > 0 && d.num_pages > 0 && d.max_pages > 0;
+    if (!context || !path || !count || !out_context || (cache && (!k_cache || !page_table)) || (k_cache && k_cache == v_cache))
+        return VKOP_INVALID_ARG;
+    const size_t esz = element_bytes(d.dtype);
+    if (misaligned(k_cache, esz) || misaligned(v_cache, esz) || misaligned(page_table, 4) || misaligned(context, 4) ||
+        misaligned(path, 4) || misaligned(count, 4) || misaligned(out_context, 4))
+        return VKOP_INVALID_ARG;
+    if (out_context < context + d.batch && context < out_context + d.batch)
+        return VKOP_INVALID_ARG;  // other blocks still read the old lengths
+    return launch_cache_compact(d, k_cache, v_cache, page_table, context, path, count, out_context,
+                                static_cast<cudaStream_t>(stream));
+}
+
 int vkop_cuda_packets_push(const void *packets, size_t packets_bytes, void *const *peer_slots, void *const *peer_flags,
                            int32_t rank, int32_t world, uint32_t seq, void *tickets, void *stream) {
     if (!packets || !peer_slots || !peer_flags || !tickets || world < 1 || world > 1024 || rank < 0 || rank >= world ||

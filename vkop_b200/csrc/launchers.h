@@ -98,6 +98,18 @@ int launch_nms(const vkop_nms_desc &d, const void *boxes, const void *scores, in
 int launch_sample_topk(const void *values, int dtype, const void *indices, int index_dtype, int64_t rows, int k, float top_p,
                        const float *u, int32_t *out_choice, void *out_token, cudaStream_t stream);
 
+// ---- speculative decoding: verification (draft_verify.cu), attention of a token tree over a paged cache
+// (tree_attention.cu), move of the accepted cache rows (cache_compact.cu) ----
+int launch_draft_verify(const vkop_draft_verify_desc &d, const void *target, const void *draft, const void *tokens,
+                        const int32_t *parents, const int32_t *num_nodes, const float *u, int32_t *out_path, int32_t *out_count,
+                        void *out_token, float *out_chance, cudaStream_t stream);
+int plan_tree_attention(const vkop_tree_attention_desc &d, size_t *bytes);
+int launch_tree_attention(const vkop_tree_attention_desc &d, const void *q, const void *k, const void *v, const int32_t *table,
+                          const int32_t *context, const int32_t *parents, const int32_t *num_nodes, void *out, float *lse,
+                          void *workspace, cudaStream_t stream);
+int launch_cache_compact(const vkop_cache_compact_desc &d, void *k, void *v, const int32_t *table, const int32_t *context,
+                         const int32_t *path, const int32_t *count, int32_t *out_context, cudaStream_t stream);
+
 // ---- packet exchange over peer memory (peer_exchange.cu) ----
 int launch_packets_push(const void *packets, size_t bytes, void *const *peer_slots, void *const *peer_flags, int rank,
                         int world, uint32_t seq, void *tickets, cudaStream_t stream);
