@@ -181,6 +181,10 @@ static TreePlan plan_general(const vkop_tree_attention_desc &d) { return plan_pa
 
 int plan_tree_attention(const vkop_tree_attention_desc &d, size_t *bytes) {
     *bytes = plan_general(d).bytes;
+    if (tree_mma_serves(d)) {  // the pointers' alignment decides at the call
+        const size_t mma = tree_mma_workspace(d);
+        *bytes = *bytes > mma ? *bytes : mma;
+    }
     return VKOP_OK;
 }
 
@@ -255,6 +259,14 @@ int launch_tree_attention(const vkop_tree_attention_desc &d, const void *q, cons
     a.max_pages = d.num_pages > 0 ? d.max_pages : 0;  // without pages the table is not looked at
     a.rows = d.nodes * a.group;
     a.scale_log2 = d.scale * kLog2e;
+    // 16-byte pieces of rows: every pointer and stride a multiple of 8 elements
+    int64_t bits = 0;
+    for (const void *p : {q, k, v, static_cast<const void *>(out)})
+        bits |= reinterpret_cast<intptr_t>(p) / 2;
+    for (int64_t s : {a.q_bs, a.q_ns, a.q_hs, a.o_bs, a.o_ns, a.o_hs, a.k_ps, a.k_ts, a.k_hs, a.v_ps, a.v_ts, a.v_hs})
+        bits |= s;
+    if (tree_mma_serves(d) && bits % 8 == 0)
+        return launch_tree_mma(a, d.dtype, workspace, stream);
     switch (d.dtype) {
     case VKOP_F32: return launch_t<float>(a, d, stream);
     case VKOP_F16: return launch_t<__half>(a, d, stream);
