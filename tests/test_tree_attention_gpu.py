@@ -81,6 +81,18 @@ def test_padding_nodes_and_empty_sequences_are_zero(capi, dim):
     assert torch.equal(wild[0], out) and torch.equal(wild[1], lse)
 
 
+@pytest.mark.parametrize("batch,kv_heads,length", [(3, 2, 1500), (40, 8, 700)])
+def test_padding_nodes_of_long_sequences(capi, batch, kv_heads, length):
+    """Few sequences, whose rows several CTAs share, and many, of which a CTA takes several in turn."""
+    g = torch.Generator().manual_seed(4)
+    used = torch.randint(0, 6, (batch,), generator=g).tolist()
+    context = torch.randint(length // 2, length, (batch,), generator=g).tolist()
+    c = case(batch, 5, kv_heads, 2, 64, 16, context, torch.float16, True, seed=8, used=used)
+    out, lse = check(capi, *c)
+    pad = torch.arange(5)[None] >= torch.tensor(used)[:, None]
+    assert (out.cpu()[pad] == 0).all() and (lse.cpu()[pad] == -INF).all()
+
+
 @pytest.mark.parametrize("dtype,dim", [(torch.float16, 64), (torch.bfloat16, 128), (torch.float32, 64)])
 def test_what_masked_places_hold_does_not_matter(capi, dtype, dim):
     """NaN and infinities behind the sequences (in every case here) and in drafted rows of other branches."""
@@ -185,6 +197,19 @@ def test_long_context_and_a_bound_that_is_too_small(capi):
     for bound in (1, 5000, 200000):
         check(capi, *c, max_context=bound)
     assert a[0].shape == (1, 3, 2, 64)
+
+
+def test_a_context_past_the_table(capi):
+    """Lengths that the table cannot hold: the positions it has are attended, the drafted ones are out of reach."""
+    for dim in (64, 80):
+        q, k, v, table, context, parents, _ = case(2, 4, 1, 2, dim, 16, [400, 90], torch.float16, True, seed=23)
+        far = torch.tensor([2**31 - 1, 100000], dtype=torch.int32)
+        table[table < 0] = 1 << 20
+        got = run(capi, q, k, v, table, far, parents)
+        pages = table.shape[1] * 16
+        # the same as a context that ends with the table, without drafted positions (their pages are not there)
+        wide = torch.cat([table, torch.full((2, 1), -1, dtype=torch.int32)], 1)
+        ref.check_attend(got, q, k, v, wide, torch.full((2,), pages, dtype=torch.int32), parents, what="past the table")
 
 
 def test_offsets_past_32_bits(capi):

@@ -41,7 +41,19 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// Arrival that also announces `bytes` that asynchronous copies will add to this phase.
+__device__ __forceinline__ void mbar_arrive_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+
 // ---- asynchronous copies ----
+// box of a four-dimensional tensor map (this GPU's memory) -> shared; its bytes count towards the barrier's phase
+__device__ __forceinline__ void copy_box(uint32_t dst, const void *map, int c0, int c1, int c2, int c3, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+        : "memory");
+}
 // 16 bytes global -> shared; nothing is read and zeros are written when bytes == 0
 __device__ __forceinline__ void copy16_or_zero(uint32_t dst, const void *src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -92,6 +104,15 @@ __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&r)[
         "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
         "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
+}
+
+// One lane of a converged warp, the same one every time.  The products are issued under this predicate, with operands that are
+// the same in the whole warp: they are kept in uniform registers then (issued under lane == 0, with the rest of the warp
+// elsewhere, a product took 300 cycles to issue instead of 64).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+    return p != 0;
 }
 
 // ---- matrix products (kind::f16: 16-bit inputs of one type, 32-bit accumulators) ----

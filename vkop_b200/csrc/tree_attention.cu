@@ -29,7 +29,7 @@ __global__ void __launch_bounds__(kGenWarps * 32) tree_attention_general_kernel(
     const int part = blockIdx.x, b = blockIdx.z;
     const int h = blockIdx.y % a.kv_heads, r = blockIdx.y / a.kv_heads * kGenWarps + warp;
     const int used = tree_used(a, b);
-    const int64_t context = tree_context(a, b), length = context + used;
+    const int64_t context = tree_context(a, b), length = tree_length(a, b);
     const int live = tree_live_parts(a, length);
     if (part >= live)
         return;
@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_attention_join_kernel(co
         return;
     const int64_t unit = row / a.rows;
     const int r = static_cast<int>(row - unit * a.rows), b = static_cast<int>(unit / a.kv_heads), h = static_cast<int>(unit % a.kv_heads);
-    const int live = tree_live_parts(a, tree_context(a, b) + tree_used(a, b));
+    const int live = tree_live_parts(a, tree_length(a, b));
     if (live == 1)
         return;
     const int64_t at = unit * a.parts * a.rows + r;

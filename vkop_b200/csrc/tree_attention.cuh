@@ -33,6 +33,12 @@ __device__ __forceinline__ int tree_used(const TreeArgs &a, int b) {
 }
 __device__ __forceinline__ int64_t tree_context(const TreeArgs &a, int b) { return max(a.context[b], 0); }
 
+// Positions to look at: those behind the table have no page.
+__device__ __forceinline__ int64_t tree_length(const TreeArgs &a, int b) {
+    const int64_t length = tree_context(a, b) + tree_used(a, b), width = static_cast<int64_t>(a.max_pages) * a.page_size;
+    return length < width ? length : width;
+}
+
 // Parts that hold positions of a sequence of this length (one at least, which writes the empty rows too).
 __device__ __forceinline__ int tree_live_parts(const TreeArgs &a, int64_t length) {
     const int64_t n = (length + a.part_tokens - 1) / a.part_tokens;

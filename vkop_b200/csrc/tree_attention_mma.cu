@@ -1,13 +1,17 @@
 // Attention of a tree of drafted tokens over a paged cache on the tensor cores: 16-bit types, head sizes 64 and 128.
 //
-// The rows that share a cache head (nodes x query heads a cache head) fill the M dimension of 128-row products; a tile of 128
-// cached positions is the N dimension of S = Q K^T and the K dimension of O += P V.  Roles of a CTA (one a SM, 16 warps):
+// The rows that share a cache head (nodes x query heads a cache head) fill the M dimension of 128-row products; 64 cached
+// positions are the N dimension of S = Q K^T and the K dimension of O += P V.  Roles of a CTA (one a SM, 16 warps):
 //   warps 0-7    softmax: two groups of 128 threads, a thread a row.  With more than 128 rows each group has its own 128 and
-//                both see every tile (ROWT = 2); otherwise the groups take the tiles in turn and their sums are joined at the
-//                end (ROWT = 1), so that one group's exponentials overlap the other's products either way.
-//   warps 8-11   copies: 16-byte asynchronous copies gather the rows of a tile from their pages into a ring of buffers in the
-//                128-byte swizzled layout that the products read (any page size, any strides; rows past the end become zeros).
-//   warp 12      one thread issues the products; S (then P in its place) and O live in tensor memory.
+//                both see every position (ROWT = 2); otherwise one group takes the first, the other the second half of every
+//                tile of 128 positions and their sums are joined at the end (ROWT = 1).
+//   warps 8-11   copies: a tile's keys and values come from their pages into a ring of buffers, in rows of 128 bytes with the
+//                128-byte swizzle that the products read.  Where 32 rows in turn are all there and belong to the context,
+//                and the page size is a power of two from 8 on, tensor-map copies of up to 32 rows bring them; the others
+//                (the end of a sequence, missing pages, other page sizes) are gathered by 16-byte copies, which leave zeros
+//                where nothing is.
+//   warps 12-13  products: one warp a softmax group.  S (then P in its place) and O live in tensor memory; two S tiles a
+//                group alternate, so that one is being made while the other is turned into weights.
 //
 // S: exponents are taken relative to a reference that follows the row's maximum only when it grows by more than 2^8 (the sums
 // are rescaled then, in tensor memory); P is scaled by 2^kBias so that 16-bit weights stay clear of the subnormal range.
@@ -19,13 +23,16 @@
 //
 // Bound: reading the cache once from HBM for few rows a head; around 256 rows the products and the exponentials
 // (16 a clock and SM) take as long as the copies.
+#include <cuda.h>
+
 #include "tensor_core.cuh"
 #include "tree_attention.cuh"
 
 namespace vkop_cuda {
 
 constexpr int kMmaThreads = 512;
-constexpr int kTile = 128;       // positions a tile
+constexpr int kTile = 128;       // positions a tile: what a buffer of the ring holds
+constexpr int kHalf = 64;        // positions a product
 constexpr int kMmaCtas = 148;
 constexpr float kBias = 6.0f;    // log2 of the scale of the weights
 constexpr float kGrow = 8.0f;    // log2 of the growth of the maximum that is let pass; 2^(6 + 8) < 65504
@@ -33,6 +40,8 @@ constexpr int kSlots = 8;        // tiles (and units) whose flags may be alive a
 
 struct TreeMmaArgs {
     TreeArgs a;
+    int box_rows;     // rows of a tensor-map copy; 0: rows are gathered one by one
+    int page_shift;   // log2(page_size), -1 where it is not a power of two
     int64_t *starts;  // [batch + 1] first tile of a sequence in the list of all tiles
     int mtiles;       // groups of ROWT * 128 rows a head
     float scale;      // |scale| * log2(e)
@@ -50,7 +59,7 @@ struct TreeMmaShape {
 };
 
 struct TreeMmaExtras {
-    uint64_t full[8], empty[8], s_ready[2], p_ready[2], pv_done[2], q_ready;
+    uint64_t full[8], empty[8], s_ready[2][2], p_ready[2][2], pv_done[2][2], q_ready;
     int64_t left;
     uint32_t tmem;
     int abort, begin_b, begin_u, begin_j, pad;
@@ -62,7 +71,7 @@ struct TreeMmaExtras {
 static_assert(sizeof(TreeMmaExtras) <= 3072, "extras");
 
 __device__ __forceinline__ int tree_tiles(const TreeArgs &a, int b) {
-    const int64_t length = tree_context(a, b) + tree_used(a, b);
+    const int64_t length = tree_length(a, b);
     return length <= 0 ? 1 : static_cast<int>((length + kTile - 1) / kTile);
 }
 
@@ -94,7 +103,7 @@ struct TreeWalk {
         if (tiles < 0) {
             context = tree_context(a, b);
             used = tree_used(a, b);
-            length = context + used;
+            length = tree_length(a, b);
             tiles = length <= 0 ? 1 : static_cast<int>((length + kTile - 1) / kTile);
         }
         j0 = j1;
@@ -106,32 +115,24 @@ struct TreeWalk {
     __device__ __forceinline__ bool whole() const { return j0 == 0 && j1 == tiles; }
 };
 
-template <int N>
-__device__ __forceinline__ void set_registers_up() {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void set_registers_down() {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-
 // ---- copies ----
 template <typename T, int D, int ROWT>
-__device__ __forceinline__ void tree_copy_role(const TreeMmaArgs &g, TreeMmaExtras &x, uint32_t ring, int units) {
+__device__ __forceinline__ void tree_copy_role(const TreeMmaArgs &g, const CUtensorMap *k_map, const CUtensorMap *v_map, TreeMmaExtras &x,
+                                               uint32_t ring, int units) {
     using Shape = TreeMmaShape<D, ROWT>;
     constexpr int NB = Shape::kRing;
     constexpr int CHUNKS = D / 8;          // 16-byte pieces of a row
-    constexpr int ROWS = 32 / CHUNKS;      // rows a warp copies at a time
+    constexpr int ROWS = 32 / CHUNKS;      // rows a warp gathers at a time
     const TreeArgs &a = g.a;
     const int lane = threadIdx.x & 31, pw = (threadIdx.x >> 5) & 3;
     const int chunk = lane % CHUNKS, sub = lane / CHUNKS;
     const uint32_t column = static_cast<uint32_t>(chunk >> 3) * (kTile * 128);
     volatile int *abort = &x.abort;
-    int next = 0;                // buffers issued so far
-    int told = 0;                // buffers announced so far: next - told <= 2 between calls
+    int next = 0;  // buffers issued so far; this warp brings rows 32 pw .. 32 pw + 31 of each
+    int told = 0;  // buffers announced so far; gathered ones follow when their copies have landed
     // a value tile with drafted rows: their values that are not finite are taken out (the epilogue adds them to the rows that
     // attend them; as a factor of a zero weight they would spoil the others)
-    int64_t check_from = 0;      // first drafted row of the tile in question, in rows of this warp
+    int check_from = 0;  // first drafted row of the buffer in question, in rows of this warp
     int check_buffer = -1, check_seg = 0;
     auto announce = [&](int upto) {
         for (; told < upto; told++) {
@@ -168,7 +169,7 @@ __device__ __forceinline__ void tree_copy_role(const TreeMmaArgs &g, TreeMmaExtr
             mbar_arrive(smem_addr(&x.full[told % NB]));
         }
     };
-    // one more buffer may be issued; announces older ones first when it has to wait
+    // the next buffer may be filled; older ones are announced first when that has to be waited for
     auto claim = [&]() {
         const uint32_t bar = smem_addr(&x.empty[next % NB]), parity = ((next / NB) & 1) ^ 1;
         if (!mbar_try(bar, parity)) {
@@ -176,8 +177,37 @@ __device__ __forceinline__ void tree_copy_role(const TreeMmaArgs &g, TreeMmaExtr
             announce(next);
             mbar_wait(bar, parity, abort);
         }
+        __syncwarp();
     };
-    auto issued = [&]() {
+    // 32 rows by tensor-map copies
+    auto boxes = [&](const CUtensorMap *map, int h, int page, int slot) {
+        if (told < next) {
+            copy_wait<0>();
+            announce(next);
+        }
+        const uint32_t bar = smem_addr(&x.full[next % NB]), buf = ring + static_cast<uint32_t>(next % NB) * Shape::kBuffer;
+        if (lane == 0)
+            mbar_arrive_expect(bar, 32 * D * 2);
+        else
+            mbar_arrive(bar);
+        const int row = lane / (D / 64) * g.box_rows;  // this lane's copy: rows from here on, one of the 64-wide column blocks
+        const int page_of = __shfl_sync(kFullMask, page, row & 31), slot_of = __shfl_sync(kFullMask, slot, row & 31);
+        if (row < 32)
+            copy_box(buf + static_cast<uint32_t>(lane % (D / 64)) * (kTile * 128) + static_cast<uint32_t>(pw * 32 + row) * 128, map,
+                     lane % (D / 64) * 64, slot_of, h, page_of, bar);
+        told = ++next;
+    };
+    // 32 rows piece by piece, zeros where `ok` has no bit
+    auto gather = [&](const T *head, int64_t at, unsigned ok) {
+        const uint32_t dst = ring + static_cast<uint32_t>(next % NB) * Shape::kBuffer + column + static_cast<uint32_t>(pw * 32 + sub) * 128;
+#pragma unroll
+        for (int i = 0; i < 32 / ROWS; i++) {
+            const int r = sub + i * ROWS;
+            const int64_t from = __shfl_sync(kFullMask, at, r);
+            const bool good = ok >> r & 1u;
+            copy16_or_zero(dst + static_cast<uint32_t>(i * ROWS) * 128 + (static_cast<uint32_t>((chunk & 7) ^ (r & 7)) << 4),
+                           good ? static_cast<const void *>(head + from) : a.q, good ? 16u : 0u);
+        }
         copy_commit();
         next++;
         if (next - told > 2) {
@@ -191,144 +221,131 @@ __device__ __forceinline__ void tree_copy_role(const TreeMmaArgs &g, TreeMmaExtr
     while (walk.next(a, units)) {
         const int h = walk.u / g.mtiles;
         const T *kh = static_cast<const T *>(a.k) + h * a.k_hs + chunk * 8, *vh = static_cast<const T *>(a.v) + h * a.v_hs + chunk * 8;
+        // this lane's row of a tile: its page (-1: none) and slot; looked up a tile ahead
+        auto look = [&](int j, int *slot) {
+            const uint32_t pos = static_cast<uint32_t>(j) * kTile + pw * 32 + lane;
+            const uint32_t page = g.page_shift >= 0 ? pos >> g.page_shift : pos / static_cast<uint32_t>(a.page_size);
+            *slot = static_cast<int>(pos - page * static_cast<uint32_t>(a.page_size));
+            return j < walk.j1 && pos < walk.length && page < static_cast<uint32_t>(a.max_pages) ? a.table[walk.b * a.table_stride + page] : -1;
+        };
+        int slot, slot_next = 0, page_next = look(walk.j0, &slot_next);
         for (int j = walk.j0; j < walk.j1; j++, tile++) {
-            const int64_t pos = static_cast<int64_t>(j) * kTile + pw * 32 + lane;
-            int slot = 0;
-            const int64_t page = pos < walk.length ? tree_page(a, walk.b, pos, &slot) : -1;
-            const unsigned ok = __ballot_sync(kFullMask, page >= 0);
-            const int64_t k_at = page * a.k_ps + slot * a.k_ts, v_at = page * a.v_ps + slot * a.v_ts;
+            const int page = page_next;
+            slot = slot_next;
+            page_next = look(j + 1, &slot_next);
+            const unsigned ok = __ballot_sync(kFullMask, page >= 0 && page < a.num_pages);
+            const int64_t drafted = walk.context - (static_cast<int64_t>(j) * kTile + pw * 32);  // first drafted row of the 32
+            const bool whole = g.box_rows > 0 && ok == kFullMask && drafted >= 32;
             claim();
             if (lane == 0)
                 x.valid[tile & (kSlots - 1)][pw] = ok;
-            uint32_t dst = ring + static_cast<uint32_t>(next % NB) * Shape::kBuffer + column + static_cast<uint32_t>(pw * 32 + sub) * 128;
-#pragma unroll
-            for (int i = 0; i < 32 / ROWS; i++) {
-                const int r = sub + i * ROWS;
-                const int64_t at = __shfl_sync(kFullMask, k_at, r);
-                const bool good = ok >> r & 1u;
-                copy16_or_zero(dst + static_cast<uint32_t>(i * ROWS) * 128 + (static_cast<uint32_t>((chunk & 7) ^ (r & 7)) << 4),
-                               good ? static_cast<const void *>(kh + at) : a.q, good ? 16u : 0u);
-            }
-            issued();
+            if (whole)
+                boxes(k_map, h, page, slot);
+            else
+                gather(kh, page * a.k_ps + slot * a.k_ts, ok);
             claim();
-            dst = ring + static_cast<uint32_t>(next % NB) * Shape::kBuffer + column + static_cast<uint32_t>(pw * 32 + sub) * 128;
-#pragma unroll
-            for (int i = 0; i < 32 / ROWS; i++) {
-                const int r = sub + i * ROWS;
-                const int64_t at = __shfl_sync(kFullMask, v_at, r);
-                const bool good = ok >> r & 1u;
-                copy16_or_zero(dst + static_cast<uint32_t>(i * ROWS) * 128 + (static_cast<uint32_t>((chunk & 7) ^ (r & 7)) << 4),
-                               good ? static_cast<const void *>(vh + at) : a.q, good ? 16u : 0u);
-            }
-            if (static_cast<int64_t>(j + 1) * kTile > walk.context) {
-                if (check_buffer >= told) {  // an earlier one is still to be announced
-                    copy_wait<0>();
-                    announce(next);
+            if (whole) {
+                boxes(v_map, h, page, slot);
+            } else {
+                if (drafted < 32) {
+                    if (check_buffer >= told) {  // an earlier one is still to be announced
+                        copy_wait<0>();
+                        announce(next);
+                    }
+                    check_buffer = next;
+                    check_from = static_cast<int>(drafted < 0 ? 0 : drafted);
+                    check_seg = walk.seg;
                 }
-                check_buffer = next;
-                check_from = walk.context - static_cast<int64_t>(j) * kTile - pw * 32;
-                check_seg = walk.seg;
+                gather(vh, page * a.v_ps + slot * a.v_ts, ok);
             }
-            issued();
         }
     }
     copy_wait<0>();
     announce(next);
+    // nothing of this CTA is in flight when it ends, not even after a wait that ran out (bounded as well)
+    volatile int gave_up = 0;
+    for (int n = next > NB ? next - NB : 0; n < next; n++)
+        mbar_wait(smem_addr(&x.full[n % NB]), (n / NB) & 1, &gave_up);
 }
 
-// ---- products ----
+// ---- products of softmax group w ----
 template <typename T, int D, int ROWT>
-__device__ __forceinline__ void tree_product_role(const TreeMmaArgs &g, TreeMmaExtras &x, uint32_t q_smem, uint32_t ring, int units) {
+__device__ __forceinline__ void tree_product_role(const TreeMmaArgs &g, TreeMmaExtras &x, uint32_t q_smem, uint32_t ring, int units, int w) {
     using Shape = TreeMmaShape<D, ROWT>;
     constexpr int NB = Shape::kRing;
-    constexpr uint32_t qk = mma_instruction<T>(128, kTile, false), pv = mma_instruction<T>(128, D, true);
+    constexpr uint32_t qk = mma_instruction<T>(128, kHalf, false), pv = mma_instruction<T>(128, D, true);
     volatile int *abort = &x.abort;
-    const uint32_t tmem = x.tmem;
-    int scores[2] = {0, 0};  // S tiles issued for a group
-    int weights[2] = {0, 0}; // P tiles multiplied
-    int first = 0;           // first buffer of the unit's tiles (keys, values, keys, ...)
+    const uint32_t tmem = __shfl_sync(kFullMask, x.tmem, 0);
+    const uint32_t t_s = tmem + w * 2 * kHalf, t_o = tmem + 4 * kHalf + w * D;
+    int made = 0;     // S tiles made
+    int weighed = 0;  // P tiles multiplied
+    int first = 0;    // first buffer of the unit's tiles (keys, values, keys, ...)
     bool ok = true;
-    auto wait_buffer = [&](int n) { ok = mbar_wait(smem_addr(&x.full[n % NB]), (n / NB) & 1, abort) && ok; };
-    auto score = [&](int w, int n) {  // S_w = Q K^T from buffer n
-        if (ok) {
-            const uint32_t qb = q_smem + (ROWT == 2 ? static_cast<uint32_t>(w) * (128 * D * 2) : 0u), kb = ring + static_cast<uint32_t>(n % NB) * Shape::kBuffer;
-            tc_fence_after();
+    auto wait = [&](uint64_t &bar, int phase) { ok = __all_sync(kFullMask, mbar_wait(smem_addr(&bar), phase & 1, abort)) && ok; };
+    auto score = [&](int n, int half, bool last) {  // next S = Q K^T from a half of buffer n, which is free after its last use
+        wait(x.full[n % NB], n / NB);
+        const uint32_t kb = __shfl_sync(kFullMask, ring + static_cast<uint32_t>(n % NB) * Shape::kBuffer + half * (kHalf * 128), 0);
+        const uint32_t to = __shfl_sync(kFullMask, t_s + (made & 1) * kHalf, 0);
+        const uint32_t qb = q_smem + (ROWT == 2 ? static_cast<uint32_t>(w) * (128 * D * 2) : 0u);
+        tc_fence_after();
+        if (elect_one()) {
+            if (ok) {
 #pragma unroll
-            for (int k = 0; k < D / 16; k++)
-                mma_ss(tmem + w * kTile, mma_operand(qb + (k >> 2) * (128 * 128) + (k & 3) * 32, 16, 1024),
-                       mma_operand(kb + (k >> 2) * (kTile * 128) + (k & 3) * 32, 16, 1024), qk, k > 0);
+                for (int k = 0; k < D / 16; k++)
+                    mma_ss(to, mma_operand(qb + (k >> 2) * (128 * 128) + (k & 3) * 32, 16, 1024),
+                           mma_operand(kb + (k >> 2) * (kTile * 128) + (k & 3) * 32, 16, 1024), qk, k > 0);
+            }
+            mma_commit(smem_addr(&x.s_ready[w][made & 1]));
+            if (last)
+                mma_commit(smem_addr(&x.empty[n % NB]));
         }
-        mma_commit(smem_addr(&x.s_ready[w]));
-        scores[w]++;
+        __syncwarp();
+        made++;
     };
-    auto weigh = [&](int w, int n, bool add) {  // O_w += P V from buffer n
-        ok = mbar_wait(smem_addr(&x.p_ready[w]), weights[w] & 1, abort) && ok;
-        if (ok) {
-            const uint32_t vb = ring + static_cast<uint32_t>(n % NB) * Shape::kBuffer;
-            tc_fence_after();
+    auto weigh = [&](int n, int half, bool add, bool last) {  // O += P V from a half of buffer n
+        wait(x.full[n % NB], n / NB);
+        wait(x.p_ready[w][weighed & 1], weighed >> 1);
+        const uint32_t vb = __shfl_sync(kFullMask, ring + static_cast<uint32_t>(n % NB) * Shape::kBuffer + half * (kHalf * 128), 0);
+        const uint32_t from = __shfl_sync(kFullMask, t_s + (weighed & 1) * kHalf, 0);
+        tc_fence_after();
+        if (elect_one()) {
+            if (ok) {
 #pragma unroll
-            for (int k = 0; k < kTile / 16; k++)
-                mma_ts(tmem + 2 * kTile + w * D, tmem + w * kTile + k * 8, mma_operand(vb + k * 2048, kTile * 128, 1024), pv, add || k > 0);
+                for (int k = 0; k < kHalf / 16; k++)
+                    mma_ts(t_o, from + k * 8, mma_operand(vb + k * 2048, kTile * 128, 1024), pv, add || k > 0);
+            }
+            mma_commit(smem_addr(&x.pv_done[w][weighed & 1]));
+            if (last)
+                mma_commit(smem_addr(&x.empty[n % NB]));
         }
-        mma_commit(smem_addr(&x.pv_done[w]));
-        weights[w]++;
+        __syncwarp();
+        weighed++;
     };
-    // P lies where the next S goes: the product that reads it has to be done
-    auto wait_weighed = [&](int w) { ok = mbar_wait(smem_addr(&x.pv_done[w]), (weights[w] - 1) & 1, abort) && ok; };
-    auto release = [&](int n) { mma_commit(smem_addr(&x.empty[n % NB])); };
+    auto wait_weighed = [&](int k) { wait(x.pv_done[w][k & 1], k >> 1); };
     TreeWalk walk;
     walk.begin(x);
     while (walk.next(g.a, units)) {
-        const int n = walk.j1 - walk.j0;
-        ok = mbar_wait(smem_addr(&x.q_ready), walk.seg & 1, abort) && ok;
-        if (ROWT == 2) {
-            wait_buffer(first);
-            score(0, first);
-            score(1, first);
-            release(first);
-            for (int t = 0; t < n; t++) {
-                const int k_next = first + 2 * t + 2, v_now = first + 2 * t + 1;
-                wait_buffer(v_now);
-#pragma unroll
-                for (int w = 0; w < 2; w++) {
-                    weigh(w, v_now, t > 0);
-                    if (w == 1)
-                        release(v_now);
-                    if (t + 1 < n) {
-                        if (w == 0)
-                            wait_buffer(k_next);
-                        wait_weighed(w);
-                        score(w, k_next);
-                        if (w == 1)
-                            release(k_next);
-                    }
-                }
-            }
-        } else {
-            for (int t = 0; t < 2 && t < n; t++) {
-                wait_buffer(first + 2 * t);
-                score(t, first + 2 * t);
-                release(first + 2 * t);
-            }
-            for (int t = 0; t < n; t++) {
-                const int w = t & 1, v_now = first + 2 * t + 1;
-                wait_buffer(v_now);
-                weigh(w, v_now, t > 1);
-                release(v_now);
-                if (t + 2 < n) {
-                    wait_buffer(first + 2 * t + 4);
-                    wait_weighed(w);
-                    score(w, first + 2 * t + 4);
-                    release(first + 2 * t + 4);
-                }
+        constexpr int PER = ROWT == 2 ? 2 : 1;  // S tiles a tile of positions
+        const int n = (walk.j1 - walk.j0) * PER;
+        auto half_of = [&](int i) { return ROWT == 2 ? i & 1 : w; };
+        auto last_of = [&](int i) { return ROWT == 1 || (i & 1); };
+        wait(x.q_ready, walk.seg);
+        for (int i = 0; i < 2 && i < n; i++)
+            score(first + i / PER * 2, half_of(i), last_of(i));
+        for (int i = 0; i < n; i++) {
+            weigh(first + i / PER * 2 + 1, half_of(i), i > 0, last_of(i));
+            if (i + 2 < n) {
+                // P lies where the next S goes: the product that reads it has to be done
+                wait_weighed(weighed - 1);
+                score(first + (i + 2) / PER * 2, half_of(i), last_of(i));
             }
         }
-        first += 2 * n;
+        first += 2 * (walk.j1 - walk.j0);
     }
     // tensor memory may be given back once nothing writes to it any more
-    for (int w = 0; w < 2; w++)
-        if (weights[w] > 0)
-            wait_weighed(w);
+    if (weighed > 1)
+        wait_weighed(weighed - 2);
+    wait_weighed(weighed - 1);
 }
 
 // ---- softmax and output ----
@@ -338,10 +355,12 @@ __device__ __forceinline__ void tree_softmax_role(const TreeMmaArgs &g, TreeMmaE
     const int tid = threadIdx.x, w = tid >> 7, trow = tid & 127;
     volatile int *abort = &x.abort;
     const uint32_t lanes = static_cast<uint32_t>((tid >> 5) & 3) << 21;  // this warp's quarter of the tensor-memory lanes
-    const uint32_t t_s = x.tmem + lanes + w * kTile, t_o = x.tmem + lanes + 2 * kTile + w * D;
-    int seen = 0;  // tiles that this group has worked on
+    const uint32_t s_base = x.tmem + lanes + w * 2 * kHalf, t_o = x.tmem + lanes + 4 * kHalf + w * D;
+    int seen = 0;  // S tiles that this group has worked on
     int tile = 0;  // tiles of the units before this one
     bool ok = true;
+    // a barrier serves every other product: its parity tells a phase from the one before and the one after
+    auto wait_weighed = [&](int k) { ok = __all_sync(kFullMask, mbar_wait(smem_addr(&x.pv_done[w][k & 1]), k >> 1 & 1, abort)) && ok; };
     TreeWalk walk;
     walk.begin(x);
     while (walk.next(a, units)) {
@@ -390,26 +409,23 @@ __device__ __forceinline__ void tree_softmax_role(const TreeMmaArgs &g, TreeMmaE
         }
 
         float m_ref = -INFINITY, l = 0.0f;  // reference of the exponents in log2 units, sum of the weights
-        int mine = 0;
-        for (int t = ROWT == 2 ? 0 : w; t < n; t += ROWT == 2 ? 1 : 2, mine++) {
-            ok = __all_sync(kFullMask, mbar_wait(smem_addr(&x.s_ready[w]), seen & 1, abort)) && ok;
-            seen++;
+        for (int i = 0; i < (ROWT == 2 ? 2 * n : n); i++, seen++) {
+            const int t = ROWT == 2 ? i >> 1 : i, half = ROWT == 2 ? i & 1 : w;
+            const uint32_t t_s = s_base + (seen & 1) * kHalf;
+            ok = __all_sync(kFullMask, mbar_wait(smem_addr(&x.s_ready[w][seen & 1]), seen >> 1 & 1, abort)) && ok;
             if (warp_live && ok) {
                 tc_fence_after();
-                uint32_t s[4][32];
-#pragma unroll
-                for (int c = 0; c < 4; c++)
-                    tmem_load32(t_s + 32 * c, s[c]);
+                uint32_t s[2][32];
+                tmem_load32(t_s, s[0]);
+                tmem_load32(t_s + 32, s[1]);
+                const int64_t t0 = static_cast<int64_t>(walk.j0 + t) * kTile + half * kHalf;
+                const uint2 there = *reinterpret_cast<const uint2 *>(&x.valid[(tile + t) & (kSlots - 1)][half * 2]);
                 tmem_wait_load();
+                tmem_settle32(s[0]);
+                tmem_settle32(s[1]);
+                if (t0 + kHalf > walk.context || (there.x & there.y) != 0xFFFFFFFFu) {
 #pragma unroll
-                for (int c = 0; c < 4; c++)
-                    tmem_settle32(s[c]);
-                const int64_t t0 = static_cast<int64_t>(walk.j0 + t) * kTile;
-                const uint4 there = *reinterpret_cast<const uint4 *>(x.valid[(tile + t) & (kSlots - 1)]);
-                if (t0 + kTile > walk.context || (there.x & there.y & there.z & there.w) != 0xFFFFFFFFu) {
-                    const uint32_t valid[4] = {there.x, there.y, there.z, there.w};
-#pragma unroll
-                    for (int c = 0; c < 4; c++) {
+                    for (int c = 0; c < 2; c++) {
                         const int64_t j = t0 + 32 * c - walk.context;  // node at the first of these positions; negative: context
                         uint32_t see = 0;
                         if (j <= -32) {
@@ -424,67 +440,69 @@ __device__ __forceinline__ void tree_softmax_role(const TreeMmaArgs &g, TreeMmaE
                             }
                             see = __funnelshift_r(lo, hi, sh);
                         }
-                        see = live ? see & valid[c] : 0u;
+                        see = live ? see & (c ? there.y : there.x) : 0u;
 #pragma unroll
-                        for (int i = 0; i < 32; i++)
-                            s[c][i] = see >> i & 1u ? s[c][i] : 0xFF800000u;
+                        for (int e = 0; e < 32; e++)
+                            s[c][e] = see >> e & 1u ? s[c][e] : 0xFF800000u;
                     }
                 }
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 0; i < 32; i++)
+                for (int e = 0; e < 32; e++)
 #pragma unroll
-                    for (int c = 0; c < 4; c++)
-                        top[c] = fmaxf(top[c], __uint_as_float(s[c][i]));
+                    for (int c = 0; c < 2; c++)
+                        top[(e & 1) * 2 + c] = fmaxf(top[(e & 1) * 2 + c], __uint_as_float(s[c][e]));
                 const float m_tile = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * g.scale;
                 if (__any_sync(kFullMask, m_tile > m_ref + kGrow)) {
                     // (also the first tile of a unit: m_ref = -inf, nothing to rescale yet)
                     const float m_new = fmaxf(m_ref, m_tile), keep = m_ref == m_new ? 1.0f : exp2_approx(m_ref - m_new);
                     m_ref = m_new;
                     l *= keep;
-                    if (mine > 0) {
-#pragma unroll
+                    if (i > 0) {
+                        wait_weighed(seen - 1);
+                        tc_fence_after();
+#pragma unroll 1
                         for (int c = 0; c < D / 32; c++) {
                             uint32_t o[32];
                             tmem_load32(t_o + 32 * c, o);
                             tmem_wait_load();
                             tmem_settle32(o);
 #pragma unroll
-                            for (int i = 0; i < 32; i++)
-                                o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+                            for (int e = 0; e < 32; e++)
+                                o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
                             tmem_store32(t_o + 32 * c, o);
                         }
                     }
                 }
                 const float off = (m_ref == -INFINITY ? 0.0f : m_ref) - kBias;
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                uint32_t p[32];
 #pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    uint32_t p[32];
-#pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        const int c = half * 2 + (i >> 4), e = (i & 15) * 2;
-                        const float p0 = exp2_approx(fmaf(__uint_as_float(s[c][e]), g.scale, -off));
-                        const float p1 = exp2_approx(fmaf(__uint_as_float(s[c][e + 1]), g.scale, -off));
-                        sum[(i & 1) * 2] += p0;
-                        sum[(i & 1) * 2 + 1] += p1;
-                        p[i] = TcType<T>::pack(p0, p1);
-                    }
-                    tmem_store32(t_s + 32 * half, p);
+                for (int e = 0; e < 32; e++) {
+                    const int c = e >> 4, at = (e & 15) * 2;
+                    const float p0 = exp2_approx(fmaf(__uint_as_float(s[c][at]), g.scale, -off));
+                    const float p1 = exp2_approx(fmaf(__uint_as_float(s[c][at + 1]), g.scale, -off));
+                    sum[(e & 1) * 2] += p0;
+                    sum[(e & 1) * 2 + 1] += p1;
+                    p[e] = TcType<T>::pack(p0, p1);
                 }
+                tmem_store32(t_s, p);
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 tmem_wait_store();
             }
             tc_fence_before();
-            mbar_arrive(smem_addr(&x.p_ready[w]));
+            mbar_arrive(smem_addr(&x.p_ready[w][seen & 1]));
         }
-        if (mine > 0)
-            ok = __all_sync(kFullMask, mbar_wait(smem_addr(&x.pv_done[w]), (seen - 1) & 1, abort)) && ok;
-        __syncwarp();
+        // the last S was made when all products but the last two were done
+        if (seen > 1)
+            wait_weighed(seen - 2);
+        wait_weighed(seen - 1);
         tc_fence_after();
 
         // ---- the unit's rows, or this CTA's part of them ----
-        float m = m_ref == -INFINITY ? -INFINITY : m_ref - kBias;
+        // a padding node's row took part with zeros where the tile was not masked: it attends nothing
+        l = live ? l : 0.0f;
+        float m = m_ref == -INFINITY || !live ? -INFINITY : m_ref - kBias;
         float f0 = 1.0f, f1 = 0.0f;
         constexpr int COLS = ROWT == 2 ? D : D / 2;  // a group's columns of the output
         if (ROWT == 1) {
@@ -497,7 +515,7 @@ __device__ __forceinline__ void tree_softmax_role(const TreeMmaArgs &g, TreeMmaE
             const float base = m == -INFINITY ? 0.0f : m;
             f0 = exp2_approx(u0.x - base);
             f1 = exp2_approx(u1.x - base);
-            l = u0.y * f0 + (n > 1 ? u1.y * f1 : 0.0f);
+            l = u0.y * f0 + u1.y * f1;
         }
         const bool whole = walk.whole();
         const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + (walk.seg > 0)) * (ROWT * 128) + (ROWT == 2 ? w * 128 : 0) + trow;
@@ -515,22 +533,20 @@ __device__ __forceinline__ void tree_softmax_role(const TreeMmaArgs &g, TreeMmaE
                     tmem_wait_load();
                     tmem_settle32(o);
                 } else {
-                    const uint32_t o0 = x.tmem + lanes + 2 * kTile + col;
+                    const uint32_t o0 = x.tmem + lanes + 4 * kHalf + col;
                     tmem_load32(o0, o);
                     tmem_wait_load();
                     tmem_settle32(o);
 #pragma unroll
                     for (int i = 0; i < 32; i++)
                         o[i] = __float_as_uint(__uint_as_float(o[i]) * f0);
-                    if (n > 1) {
-                        uint32_t o2[32];
-                        tmem_load32(o0 + D, o2);
-                        tmem_wait_load();
-                        tmem_settle32(o2);
+                    uint32_t o2[32];
+                    tmem_load32(o0 + D, o2);
+                    tmem_wait_load();
+                    tmem_settle32(o2);
 #pragma unroll
-                        for (int i = 0; i < 32; i++)
-                            o[i] = __float_as_uint(fmaf(__uint_as_float(o2[i]), f1, __uint_as_float(o[i])));
-                    }
+                    for (int i = 0; i < 32; i++)
+                        o[i] = __float_as_uint(fmaf(__uint_as_float(o2[i]), f1, __uint_as_float(o[i])));
                 }
                 if (row_ok) {
 #pragma unroll
@@ -594,7 +610,8 @@ __device__ __forceinline__ void tree_softmax_role(const TreeMmaArgs &g, TreeMmaE
 }
 
 template <typename T, int D, int ROWT>
-__global__ void __launch_bounds__(kMmaThreads, 1) tree_attention_mma_kernel(const TreeMmaArgs g) {
+__global__ void __launch_bounds__(kMmaThreads, 1) tree_attention_mma_kernel(const TreeMmaArgs g, const __grid_constant__ CUtensorMap k_map,
+                                                                       const __grid_constant__ CUtensorMap v_map) {
     using Shape = TreeMmaShape<D, ROWT>;
     extern __shared__ __align__(1024) unsigned char smem[];
     TreeMmaExtras &x = *reinterpret_cast<TreeMmaExtras *>(smem + Shape::kQ + Shape::kRing * Shape::kBuffer);
@@ -620,12 +637,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_attention_mma_kernel(cons
     if (tid == 0) {
         for (int i = 0; i < 8; i++) {
             mbar_init(smem_addr(&x.full[i]), 128);
-            mbar_init(smem_addr(&x.empty[i]), 1);
+            mbar_init(smem_addr(&x.empty[i]), 2);
         }
         for (int i = 0; i < 2; i++) {
-            mbar_init(smem_addr(&x.s_ready[i]), 1);
-            mbar_init(smem_addr(&x.p_ready[i]), 128);
-            mbar_init(smem_addr(&x.pv_done[i]), 1);
+            for (int k = 0; k < 2; k++) {
+                mbar_init(smem_addr(&x.s_ready[i][k]), 1);
+                mbar_init(smem_addr(&x.p_ready[i][k]), 128);
+                mbar_init(smem_addr(&x.pv_done[i][k]), 1);
+            }
         }
         mbar_init(smem_addr(&x.q_ready), 256);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -671,21 +690,12 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_attention_mma_kernel(cons
     tc_fence_after();
     const uint32_t q_smem = smem_addr(smem), ring = q_smem + Shape::kQ;
 
-    // registers: 128 a thread at launch, 2 x 184 + 88 + 56 = 4 x 128
-    if (warp < 8) {
-        set_registers_up<184>();
+    if (warp < 8)
         tree_softmax_role<T, D, ROWT>(g, x, smem, units);
-    } else if (warp < 12) {
-        set_registers_down<88>();
-        tree_copy_role<T, D, ROWT>(g, x, ring, units);
-    } else {
-        set_registers_down<56>();
-        if (warp == 12) {
-            if (lane == 0)
-                tree_product_role<T, D, ROWT>(g, x, q_smem, ring, units);
-            __syncwarp();
-        }
-    }
+    else if (warp < 12)
+        tree_copy_role<T, D, ROWT>(g, &k_map, &v_map, x, ring, units);
+    else if (warp < 14)
+        tree_product_role<T, D, ROWT>(g, x, q_smem, ring, units, warp - 12);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -763,13 +773,13 @@ size_t tree_mma_workspace(const vkop_tree_attention_desc &d) {
 }
 
 template <typename T, int D, int ROWT>
-static int launch_mma_t(const TreeMmaArgs &g, cudaStream_t stream) {
+static int launch_mma_t(const TreeMmaArgs &g, const CUtensorMap *maps, cudaStream_t stream) {
     constexpr int smem = TreeMmaShape<D, ROWT>::kSmem;
     if (cudaFuncSetAttribute(tree_attention_mma_kernel<T, D, ROWT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
         cudaGetLastError();
         return VKOP_CUDA_ERROR;
     }
-    tree_attention_mma_kernel<T, D, ROWT><<<kMmaCtas, kMmaThreads, smem, stream>>>(g);
+    tree_attention_mma_kernel<T, D, ROWT><<<kMmaCtas, kMmaThreads, smem, stream>>>(g, maps[0], maps[1]);
     note_launch();
     if (check_launch() != VKOP_OK)
         return VKOP_CUDA_ERROR;
@@ -792,10 +802,34 @@ static int launch_mma_t(const TreeMmaArgs &g, cudaStream_t stream) {
 }
 
 template <typename T>
-static int launch_mma_type(const TreeMmaArgs &g, cudaStream_t stream) {
+static int launch_mma_type(const TreeMmaArgs &g, const CUtensorMap *maps, cudaStream_t stream) {
     if (g.a.head_dim == 64)
-        return g.a.rows > 128 ? launch_mma_t<T, 64, 2>(g, stream) : launch_mma_t<T, 64, 1>(g, stream);
-    return g.a.rows > 128 ? launch_mma_t<T, 128, 2>(g, stream) : launch_mma_t<T, 128, 1>(g, stream);
+        return g.a.rows > 128 ? launch_mma_t<T, 64, 2>(g, maps, stream) : launch_mma_t<T, 64, 1>(g, maps, stream);
+    return g.a.rows > 128 ? launch_mma_t<T, 128, 2>(g, maps, stream) : launch_mma_t<T, 128, 1>(g, maps, stream);
+}
+
+// The cache as a tensor [page, head, slot, element] for copies of `rows` x 64 elements.  False where the driver has no such map.
+static bool cache_map(CUtensorMap *map, int dtype, const void *base, int64_t num_pages, int64_t ps, int64_t ts, int64_t hs, const TreeArgs &a, int rows) {
+    using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            fn = nullptr;
+        }
+        return reinterpret_cast<Encode>(fn);
+    }();
+    if (!encode)
+        return false;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.head_dim), static_cast<cuuint64_t>(a.page_size), static_cast<cuuint64_t>(a.kv_heads),
+                                static_cast<cuuint64_t>(num_pages)};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(ts) * 2, static_cast<cuuint64_t>(hs) * 2, static_cast<cuuint64_t>(ps) * 2};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows), 1, 1}, steps[4] = {1, 1, 1, 1};
+    return encode(map, dtype == VKOP_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, strides,
+                  box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 int launch_tree_mma(const TreeArgs &args, int dtype, void *workspace, cudaStream_t stream) {
@@ -809,7 +843,16 @@ int launch_tree_mma(const TreeArgs &args, int dtype, void *workspace, cudaStream
     g.scale = args.scale_log2 == 0.0f ? 1.0f : fabsf(args.scale_log2);
     g.mask = args.scale_log2 == 0.0f ? 0u : 0xFFFFFFFFu;
     g.flip = args.scale_log2 < 0.0f ? 0x80008000u : 0u;
-    return dtype == VKOP_F16 ? launch_mma_type<__half>(g, stream) : launch_mma_type<__nv_bfloat16>(g, stream);
+    g.page_shift = (args.page_size & (args.page_size - 1)) == 0 ? __builtin_ctz(static_cast<unsigned>(args.page_size)) : -1;
+    CUtensorMap maps[2] = {};
+    g.box_rows = 0;
+    if (g.page_shift >= 3 && args.max_pages > 0) {
+        const int rows = args.page_size < 32 ? args.page_size : 32;
+        if (cache_map(&maps[0], dtype, args.k, args.num_pages, args.k_ps, args.k_ts, args.k_hs, args, rows) &&
+            cache_map(&maps[1], dtype, args.v, args.num_pages, args.v_ps, args.v_ts, args.v_hs, args, rows))
+            g.box_rows = rows;
+    }
+    return dtype == VKOP_F16 ? launch_mma_type<__half>(g, maps, stream) : launch_mma_type<__nv_bfloat16>(g, maps, stream);
 }
 
 }  // namespace vkop_cuda
