@@ -11,7 +11,9 @@
 //                (the end of a sequence, missing pages, other page sizes) are gathered by 16-byte copies, which leave zeros
 //                where nothing is.
 //   warps 12-13  products: one warp a softmax group.  S (then P in its place) and O live in tensor memory; two S tiles a
-//                group alternate, so that one is being made while the other is turned into weights.
+//                group alternate, so that one is being made while the other is turned into weights.  The products of a warp
+//                are carried out in the order of their issue: the S that overwrites a P is issued behind the product that
+//                reads it, without a wait in between (with one: 2050 cycles for 64 positions).
 //
 // S: exponents are taken relative to a reference that follows the row's maximum only when it grows by more than 2^8 (the sums
 // are rescaled then, in tensor memory); P is scaled by 2^kBias so that 16-bit weights stay clear of the subnormal range.
@@ -59,7 +61,7 @@ struct TreeMmaShape {
 };
 
 struct TreeMmaExtras {
-    uint64_t full[8], empty[8], s_ready[2][2], p_ready[2][2], pv_done[2][2], q_ready;
+    uint64_t full[8], empty[8], s_ready[2][2], p_ready[2][2], pv_done[2][2], q_ready, done[2];
     int64_t left;
     uint32_t tmem;
     int abort, begin_b, begin_u, begin_j, pad;
@@ -130,19 +132,22 @@ __device__ __forceinline__ void tree_copy_role(const TreeMmaArgs &g, const CUten
     volatile int *abort = &x.abort;
     int next = 0;  // buffers issued so far; this warp brings rows 32 pw .. 32 pw + 31 of each
     int told = 0;  // buffers announced so far; gathered ones follow when their copies have landed
+    uint32_t boxed = 0;  // ring places whose buffer announces itself
     // a value tile with drafted rows: their values that are not finite are taken out (the epilogue adds them to the rows that
     // attend them; as a factor of a zero weight they would spoil the others)
-    int check_from = 0;  // first drafted row of the buffer in question, in rows of this warp
+    int check_from = 0, check_to = 0;  // drafted rows of the buffer in question, in rows of this warp
     int check_buffer = -1, check_seg = 0;
     auto announce = [&](int upto) {
         for (; told < upto; told++) {
-            const uint32_t buf = ring + static_cast<uint32_t>(told % NB) * Shape::kBuffer;
+            const int place = told % NB;
+            if (boxed >> place & 1u) {
+                boxed &= ~(1u << place);
+                continue;
+            }
+            const uint32_t buf = ring + static_cast<uint32_t>(place) * Shape::kBuffer;
             if (told == check_buffer) {
 #pragma unroll 1
-                for (int i = 0; i < 32 / ROWS; i++) {
-                    const int r = sub + i * ROWS;
-                    if (r < check_from)
-                        continue;
+                for (int r = sub + (max(check_from - sub, 0) + ROWS - 1) / ROWS * ROWS; r < check_to; r += ROWS) {
                     const uint32_t at = buf + column + static_cast<uint32_t>(pw * 32 + r) * 128 + (static_cast<uint32_t>((chunk & 7) ^ (r & 7)) << 4);
                     uint32_t v[4];
                     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at));
@@ -166,7 +171,7 @@ __device__ __forceinline__ void tree_copy_role(const TreeMmaArgs &g, const CUten
                 }
             }
             fence_proxy_async();
-            mbar_arrive(smem_addr(&x.full[told % NB]));
+            mbar_arrive(smem_addr(&x.full[place]));
         }
     };
     // the next buffer may be filled; older ones are announced first when that has to be waited for
@@ -179,12 +184,16 @@ __device__ __forceinline__ void tree_copy_role(const TreeMmaArgs &g, const CUten
         }
         __syncwarp();
     };
+    auto issued = [&]() {  // a buffer is a group of copies, a self-announcing one an empty group
+        copy_commit();
+        next++;
+        if (next - told > 2) {
+            copy_wait<2>();
+            announce(next - 2);
+        }
+    };
     // 32 rows by tensor-map copies
     auto boxes = [&](const CUtensorMap *map, int h, int page, int slot) {
-        if (told < next) {
-            copy_wait<0>();
-            announce(next);
-        }
         const uint32_t bar = smem_addr(&x.full[next % NB]), buf = ring + static_cast<uint32_t>(next % NB) * Shape::kBuffer;
         if (lane == 0)
             mbar_arrive_expect(bar, 32 * D * 2);
@@ -195,7 +204,8 @@ __device__ __forceinline__ void tree_copy_role(const TreeMmaArgs &g, const CUten
         if (row < 32)
             copy_box(buf + static_cast<uint32_t>(lane % (D / 64)) * (kTile * 128) + static_cast<uint32_t>(pw * 32 + row) * 128, map,
                      lane % (D / 64) * 64, slot_of, h, page_of, bar);
-        told = ++next;
+        boxed |= 1u << (next % NB);
+        issued();
     };
     // 32 rows piece by piece, zeros where `ok` has no bit
     auto gather = [&](const T *head, int64_t at, unsigned ok) {
@@ -208,12 +218,7 @@ __device__ __forceinline__ void tree_copy_role(const TreeMmaArgs &g, const CUten
             copy16_or_zero(dst + static_cast<uint32_t>(i * ROWS) * 128 + (static_cast<uint32_t>((chunk & 7) ^ (r & 7)) << 4),
                            good ? static_cast<const void *>(head + from) : a.q, good ? 16u : 0u);
         }
-        copy_commit();
-        next++;
-        if (next - told > 2) {
-            copy_wait<2>();
-            announce(next - 2);
-        }
+        issued();
     };
     TreeWalk walk;
     walk.begin(x);
@@ -253,7 +258,9 @@ __device__ __forceinline__ void tree_copy_role(const TreeMmaArgs &g, const CUten
                         announce(next);
                     }
                     check_buffer = next;
+                    const int64_t rows = walk.length - (static_cast<int64_t>(j) * kTile + pw * 32);
                     check_from = static_cast<int>(drafted < 0 ? 0 : drafted);
+                    check_to = static_cast<int>(rows < 0 ? 0 : rows < 32 ? rows : 32);
                     check_seg = walk.seg;
                 }
                 gather(vh, page * a.v_ps + slot * a.v_ts, ok);
@@ -284,8 +291,8 @@ __device__ __forceinline__ void tree_product_role(const TreeMmaArgs &g, TreeMmaE
     auto wait = [&](uint64_t &bar, int phase) { ok = __all_sync(kFullMask, mbar_wait(smem_addr(&bar), phase & 1, abort)) && ok; };
     auto score = [&](int n, int half, bool last) {  // next S = Q K^T from a half of buffer n, which is free after its last use
         wait(x.full[n % NB], n / NB);
-        const uint32_t kb = __shfl_sync(kFullMask, ring + static_cast<uint32_t>(n % NB) * Shape::kBuffer + half * (kHalf * 128), 0);
         const uint32_t to = __shfl_sync(kFullMask, t_s + (made & 1) * kHalf, 0);
+        const uint32_t kb = __shfl_sync(kFullMask, ring + static_cast<uint32_t>(n % NB) * Shape::kBuffer + half * (kHalf * 128), 0);
         const uint32_t qb = q_smem + (ROWT == 2 ? static_cast<uint32_t>(w) * (128 * D * 2) : 0u);
         tc_fence_after();
         if (elect_one()) {
@@ -321,7 +328,6 @@ __device__ __forceinline__ void tree_product_role(const TreeMmaArgs &g, TreeMmaE
         __syncwarp();
         weighed++;
     };
-    auto wait_weighed = [&](int k) { wait(x.pv_done[w][k & 1], k >> 1); };
     TreeWalk walk;
     walk.begin(x);
     while (walk.next(g.a, units)) {
@@ -334,18 +340,17 @@ __device__ __forceinline__ void tree_product_role(const TreeMmaArgs &g, TreeMmaE
             score(first + i / PER * 2, half_of(i), last_of(i));
         for (int i = 0; i < n; i++) {
             weigh(first + i / PER * 2 + 1, half_of(i), i > 0, last_of(i));
-            if (i + 2 < n) {
-                // P lies where the next S goes: the product that reads it has to be done
-                wait_weighed(weighed - 1);
+            if (i + 2 < n)
                 score(first + (i + 2) / PER * 2, half_of(i), last_of(i));
-            }
         }
         first += 2 * (walk.j1 - walk.j0);
     }
     // tensor memory may be given back once nothing writes to it any more
-    if (weighed > 1)
-        wait_weighed(weighed - 2);
-    wait_weighed(weighed - 1);
+    if (elect_one())
+        mma_commit(smem_addr(&x.done[w]));
+    __syncwarp();
+    volatile int gave_up = 0;
+    mbar_wait(smem_addr(&x.done[w]), 0, &gave_up);
 }
 
 // ---- softmax and output ----
@@ -359,43 +364,50 @@ __device__ __forceinline__ void tree_softmax_role(const TreeMmaArgs &g, TreeMmaE
     int seen = 0;  // S tiles that this group has worked on
     int tile = 0;  // tiles of the units before this one
     bool ok = true;
+    auto wait = [&](uint64_t &bar, int phase) { ok = __all_sync(kFullMask, mbar_wait(smem_addr(&bar), phase & 1, abort)) && ok; };
     // a barrier serves every other product: its parity tells a phase from the one before and the one after
-    auto wait_weighed = [&](int k) { ok = __all_sync(kFullMask, mbar_wait(smem_addr(&x.pv_done[w][k & 1]), k >> 1 & 1, abort)) && ok; };
-    TreeWalk walk;
-    walk.begin(x);
-    while (walk.next(a, units)) {
-        const int b = walk.b, h = walk.u / g.mtiles, n = walk.j1 - walk.j0;
-        const int row = walk.u % g.mtiles * (ROWT * 128) + (ROWT == 2 ? w * 128 : 0) + trow;
+    auto wait_weighed = [&](int k) { wait(x.pv_done[w][k & 1], k >> 1); };
+    auto row_of = [&](const TreeWalk &at) { return at.u % g.mtiles * (ROWT * 128) + (ROWT == 2 ? w * 128 : 0) + trow; };
+    // queries and parents of a unit into shared memory
+    auto load_unit = [&](const TreeWalk &at) {
+        if (static_cast<int64_t>(at.j1) * kTile > at.context && trow < a.nodes) {
+            const int up = a.parents ? a.parents[static_cast<int64_t>(at.b) * a.nodes + trow] : trow - 1;
+            x.parents[w][trow] = up >= 0 && up < trow ? up : 255;
+        }
+        constexpr int PIECES = ROWT == 2 ? D / 8 : D / 16;
+        const int from = ROWT == 2 ? 0 : w * PIECES, row = row_of(at), node = row / a.group;
+        const bool live = row < a.rows && node < at.used;
+        const T *src = static_cast<const T *>(a.q) + at.b * a.q_bs + node * a.q_ns + (at.u / g.mtiles * a.group + row % a.group) * a.q_hs;
+        unsigned char *dst = q_ptr + (ROWT == 2 ? w * (128 * D * 2) : 0) + trow * 128;
+        uint4 q[PIECES];  // all loads first: the stores below would hold the next load back
+#pragma unroll
+        for (int c = 0; c < PIECES; c++)
+            q[c] = live ? *reinterpret_cast<const uint4 *>(src + (from + c) * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int c = 0; c < PIECES; c++) {
+            const int piece = from + c;
+            uint4 v = q[c];
+            v.x = (v.x ^ g.flip) & g.mask, v.y = (v.y ^ g.flip) & g.mask, v.z = (v.z ^ g.flip) & g.mask, v.w = (v.w ^ g.flip) & g.mask;
+            *reinterpret_cast<uint4 *>(dst + (piece >> 3) * (128 * 128) + (((piece & 7) ^ (trow & 7)) << 4)) = v;
+        }
+        fence_proxy_async();
+        mbar_arrive(smem_addr(&x.q_ready));
+    };
+    TreeWalk ahead;
+    ahead.begin(x);
+    bool more = ahead.next(a, units);
+    if (more)
+        load_unit(ahead);
+    while (more) {
+        const TreeWalk walk = ahead;
+        const int b = walk.b, h = walk.u / g.mtiles, n = walk.j1 - walk.j0, row = row_of(walk);
         const bool row_ok = row < a.rows;
         const int node = row_ok ? row / a.group : 0, head = h * a.group + (row_ok ? row % a.group : 0);
         const bool live = row_ok && node < walk.used;
         const bool warp_live = __any_sync(kFullMask, live);
-        const bool drafted = static_cast<int64_t>(walk.j1) * kTile > walk.context;
-        if (drafted && trow < a.nodes) {
-            const int up = a.parents ? a.parents[static_cast<int64_t>(b) * a.nodes + trow] : trow - 1;
-            x.parents[w][trow] = up >= 0 && up < trow ? up : 255;
-        }
-        // both groups are done with the unit before: its queries (every S has been made) and its flags may go
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        if (tid == 0 && walk.seg > 0)
-            x.bad[(walk.seg - 1) & (kSlots - 1)] = 0;
-        {
-            constexpr int PIECES = ROWT == 2 ? D / 8 : D / 16;
-            const int from = ROWT == 2 ? 0 : w * PIECES;
-            const T *src = static_cast<const T *>(a.q) + b * a.q_bs + node * a.q_ns + head * a.q_hs;
-            unsigned char *dst = q_ptr + (ROWT == 2 ? w * (128 * D * 2) : 0) + trow * 128;
-#pragma unroll
-            for (int c = 0; c < PIECES; c++) {
-                const int piece = from + c;
-                uint4 v = live ? *reinterpret_cast<const uint4 *>(src + piece * 8) : make_uint4(0, 0, 0, 0);
-                v.x = (v.x ^ g.flip) & g.mask, v.y = (v.y ^ g.flip) & g.mask, v.z = (v.z ^ g.flip) & g.mask, v.w = (v.w ^ g.flip) & g.mask;
-                *reinterpret_cast<uint4 *>(dst + (piece >> 3) * (128 * 128) + (((piece & 7) ^ (trow & 7)) << 4)) = v;
-            }
-        }
-        fence_proxy_async();
-        mbar_arrive(smem_addr(&x.q_ready));
+        wait(x.q_ready, walk.seg);
         uint32_t anc[kTreeWords] = {};
-        if (drafted && live) {
+        if (static_cast<int64_t>(walk.j1) * kTile > walk.context && live) {
             int at = node;
             while (true) {
 #pragma unroll
@@ -412,7 +424,7 @@ __device__ __forceinline__ void tree_softmax_role(const TreeMmaArgs &g, TreeMmaE
         for (int i = 0; i < (ROWT == 2 ? 2 * n : n); i++, seen++) {
             const int t = ROWT == 2 ? i >> 1 : i, half = ROWT == 2 ? i & 1 : w;
             const uint32_t t_s = s_base + (seen & 1) * kHalf;
-            ok = __all_sync(kFullMask, mbar_wait(smem_addr(&x.s_ready[w][seen & 1]), seen >> 1 & 1, abort)) && ok;
+            wait(x.s_ready[w][seen & 1], seen >> 1);
             if (warp_live && ok) {
                 tc_fence_after();
                 uint32_t s[2][32];
@@ -493,23 +505,19 @@ __device__ __forceinline__ void tree_softmax_role(const TreeMmaArgs &g, TreeMmaE
             tc_fence_before();
             mbar_arrive(smem_addr(&x.p_ready[w][seen & 1]));
         }
-        // the last S was made when all products but the last two were done
-        if (seen > 1)
-            wait_weighed(seen - 2);
-        wait_weighed(seen - 1);
-        tc_fence_after();
-
         // ---- the unit's rows, or this CTA's part of them ----
         // a padding node's row took part with zeros where the tile was not masked: it attends nothing
         l = live ? l : 0.0f;
         float m = m_ref == -INFINITY || !live ? -INFINITY : m_ref - kBias;
+        if (ROWT == 1)
+            x.ml[w][trow] = make_float2(m, l);
+        // every S of the unit has been read: the next unit's queries may take the place of its queries
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (tid == 0 && walk.seg > 0)
+            x.bad[(walk.seg - 1) & (kSlots - 1)] = 0;  // the epilogue before is over
         float f0 = 1.0f, f1 = 0.0f;
         constexpr int COLS = ROWT == 2 ? D : D / 2;  // a group's columns of the output
         if (ROWT == 1) {
-            x.ml[w][trow] = make_float2(m, l);
-            tc_fence_before();
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            tc_fence_after();
             const float2 u0 = x.ml[0][trow], u1 = x.ml[1][trow];
             m = fmaxf(u0.x, u1.x);
             const float base = m == -INFINITY ? 0.0f : m;
@@ -517,6 +525,17 @@ __device__ __forceinline__ void tree_softmax_role(const TreeMmaArgs &g, TreeMmaE
             f1 = exp2_approx(u1.x - base);
             l = u0.y * f0 + u1.y * f1;
         }
+        more = ahead.next(a, units);
+        if (more)
+            load_unit(ahead);
+        if (seen > 1)
+            wait_weighed(seen - 2);
+        wait_weighed(seen - 1);
+        if (ROWT == 1) {  // each group reads the other's sums too
+            tc_fence_before();
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+        }
+        tc_fence_after();
         const bool whole = walk.whole();
         const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + (walk.seg > 0)) * (ROWT * 128) + (ROWT == 2 ? w * 128 : 0) + trow;
         T *o_row = static_cast<T *>(a.out) + b * a.o_bs + node * a.o_ns + head * a.o_hs;
@@ -591,8 +610,10 @@ __device__ __forceinline__ void tree_softmax_role(const TreeMmaArgs &g, TreeMmaE
                         }
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4)
-                            *reinterpret_cast<uint4 *>(a.part_o + slot * D + col + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        for (int i = 0; i < 32; i += 8)  // whole sectors
+                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(a.part_o + slot * D + col + i), "r"(o[i]),
+                                         "r"(o[i + 1]), "r"(o[i + 2]), "r"(o[i + 3]), "r"(o[i + 4]), "r"(o[i + 5]), "r"(o[i + 6]), "r"(o[i + 7])
+                                         : "memory");
                     }
                 }
                 __syncwarp();
@@ -606,6 +627,8 @@ __device__ __forceinline__ void tree_softmax_role(const TreeMmaArgs &g, TreeMmaE
         }
         tile += n;
         tc_fence_before();  // the next unit's products may overwrite what was read
+        if (ROWT == 1)
+            asm volatile("bar.sync 1, 256;" ::: "memory");
     }
 }
 
@@ -624,8 +647,12 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_attention_mma_kernel(cons
     const int per = (a.batch + kMmaThreads - 1) / kMmaThreads;
     const int b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
     int64_t sum = 0;
-    for (int b = b0; b < b1; b++)
-        sum += static_cast<int64_t>(tree_tiles(a, b)) * units;
+    int tiles0 = 0;  // of this thread's first sequence
+    for (int b = b0; b < b1; b++) {
+        const int tiles = tree_tiles(a, b);
+        tiles0 = b == b0 ? tiles : tiles0;
+        sum += static_cast<int64_t>(tiles) * units;
+    }
     int64_t upto = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -640,6 +667,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_attention_mma_kernel(cons
             mbar_init(smem_addr(&x.empty[i]), 2);
         }
         for (int i = 0; i < 2; i++) {
+            mbar_init(smem_addr(&x.done[i]), 1);
             for (int k = 0; k < 2; k++) {
                 mbar_init(smem_addr(&x.s_ready[i][k]), 1);
                 mbar_init(smem_addr(&x.p_ready[i][k]), 128);
@@ -664,14 +692,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_attention_mma_kernel(cons
         int64_t at = before;
         for (int b = b0; b < b1; b++) {
             g.starts[b] = at;
-            at += static_cast<int64_t>(tree_tiles(a, b)) * units;
+            at += static_cast<int64_t>(b == b0 ? tiles0 : tree_tiles(a, b)) * units;
         }
         if (tid == 0)
             g.starts[a.batch] = total;
     }
     if (lo < hi && lo >= before && lo < before + sum) {
         int64_t at = before;
-        int b = b0, tiles = tree_tiles(a, b);
+        int b = b0, tiles = tiles0;
         while (lo >= at + static_cast<int64_t>(tiles) * units) {
             at += static_cast<int64_t>(tiles) * units;
             tiles = tree_tiles(a, ++b);
@@ -720,34 +748,41 @@ __global__ void __launch_bounds__(kMmaJoinWarps * 32) tree_attention_mma_join_ke
     const int c0 = static_cast<int>(((lo + 1) * ctas - 1) / total), c1 = static_cast<int>((hi * ctas - 1) / total);
     if (c0 == c1)
         return;  // written out by the one CTA
-    // CTA c's part lies in its first slot when its range begins inside the unit, else in its second; a range may be empty
-    auto part = [&](int c) -> int64_t {
-        const int64_t from = c * total / ctas;
-        if (from == (c + 1) * total / ctas)
-            return -1;
-        return (static_cast<int64_t>(c) * 2 + (from < lo)) * (ROWT * 128) + in_unit;
-    };
-    float top = -INFINITY;
-    for (int c = c0 + lane; c <= c1; c += 32)
-        if (const int64_t i = part(c); i >= 0)
-            top = fmaxf(top, a.part_ml[i].x);
-    top = warp_max(top);
-    const float base = top == -INFINITY ? 0.0f : top;
-    float l = 0.0f, acc[D / 32];
+    // CTA c's part lies in its first slot when its range begins inside the unit, else in its second; a range may be empty.
+    // The lanes look 32 parts up at a time; parts are added in the order of the CTAs.
+    float top = -INFINITY, l = 0.0f, acc[D / 32];
 #pragma unroll
     for (int e = 0; e < D / 32; e++)
         acc[e] = 0.0f;
-#pragma unroll 4
-    for (int c = c0; c <= c1; c++) {
-        const int64_t i = part(c);
-        if (i < 0)
-            continue;
-        const float2 ml = a.part_ml[i];
+    for (int c = c0; c <= c1; c += 32) {
+        const int mine = c + lane;
+        int slot = -1;
+        float2 ml = make_float2(-INFINITY, 0.0f);
+        if (mine <= c1) {
+            const int64_t from = mine * total / ctas;
+            if (from != (mine + 1) * total / ctas) {
+                slot = (mine * 2 + (from < lo)) * (ROWT * 128) + in_unit;
+                ml = a.part_ml[slot];
+            }
+        }
+        const float higher = fmaxf(top, warp_max(ml.x)), base = higher == -INFINITY ? 0.0f : higher, keep = exp2f(top - base);
         const float f = exp2f(ml.x - base);
-        l = fmaf(f, ml.y, l);
+        top = higher;
+        l = l * keep + warp_sum(f * ml.y);
 #pragma unroll
         for (int e = 0; e < D / 32; e++)
-            acc[e] = fmaf(f, a.part_o[i * D + lane + 32 * e], acc[e]);
+            acc[e] *= keep;
+        const int count = min(32, c1 - c + 1);
+#pragma unroll 8
+        for (int p = 0; p < count; p++) {
+            const int at = __shfl_sync(kFullMask, slot, p);
+            const float w = __shfl_sync(kFullMask, f, p);
+            if (at < 0)
+                continue;
+#pragma unroll
+            for (int e = 0; e < D / 32; e++)
+                acc[e] = fmaf(w, a.part_o[static_cast<int64_t>(at) * D + lane + 32 * e], acc[e]);
+        }
     }
     const int node = row / a.group, head = u / g.mtiles * a.group + row % a.group;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -768,7 +803,7 @@ static int64_t slot_rows(const TreeArgs &a) { return a.rows > 128 ? 256 : 128; }
 
 size_t tree_mma_workspace(const vkop_tree_attention_desc &d) {
     const int64_t rows = static_cast<int64_t>(d.nodes) * (d.q_heads / d.kv_heads) > 128 ? 256 : 128;
-    const size_t starts = (static_cast<size_t>(d.batch + 1) * 8 + 15) / 16 * 16;
+    const size_t starts = (static_cast<size_t>(d.batch + 1) * 8 + 31) / 32 * 32 + 32;
     return starts + static_cast<size_t>(kMmaCtas) * 2 * rows * (d.head_dim + 2) * sizeof(float);
 }
 
@@ -835,8 +870,9 @@ static bool cache_map(CUtensorMap *map, int dtype, const void *base, int64_t num
 int launch_tree_mma(const TreeArgs &args, int dtype, void *workspace, cudaStream_t stream) {
     TreeMmaArgs g;
     g.a = args;
+    workspace = reinterpret_cast<void *>((reinterpret_cast<uintptr_t>(workspace) + 31) / 32 * 32);  // the parts are stored 32 bytes at a time
     g.starts = static_cast<int64_t *>(workspace);
-    const size_t starts = (static_cast<size_t>(args.batch + 1) * 8 + 15) / 16 * 16;
+    const size_t starts = (static_cast<size_t>(args.batch + 1) * 8 + 31) / 32 * 32;
     g.a.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + starts);
     g.a.part_o = reinterpret_cast<float *>(g.a.part_ml + kMmaCtas * 2 * slot_rows(args));
     g.mtiles = args.rows > 128 ? (args.rows + 255) / 256 : 1;
