@@ -10,7 +10,8 @@
 //                and the page size is a power of two from 8 on, tensor-map copies of up to 32 rows bring them; the others
 //                (the end of a sequence, missing pages, other page sizes) are gathered by 16-byte copies, which leave zeros
 //                where nothing is.
-//   warps 12-13  products: one warp a softmax group.  S (then P in its place) and O live in tensor memory; two S tiles a
+//   warp 12      products, for the groups in turn (two warps that issue at the same time let the groups wait for each
+//                other's products: 1900 cycles for 64 positions of 256 rows against 1850, and 53 us against 51 for 26 rows of 64).  S (then P in its place) and O live in tensor memory; two S tiles a
 //                group alternate, so that one is being made while the other is turned into weights.  The products of a warp
 //                are carried out in the order of their issue: the S that overwrites a P is issued behind the product that
 //                reads it, without a wait in between (with one: 2050 cycles for 64 positions).
@@ -44,7 +45,7 @@ struct TreeMmaArgs {
     TreeArgs a;
     int box_rows;     // rows of a tensor-map copy; 0: rows are gathered one by one
     int page_shift;   // log2(page_size), -1 where it is not a power of two
-    int64_t *starts;  // [batch + 1] first tile of a sequence in the list of all tiles
+    int64_t *starts;  // [batch + 1] first place of a sequence in the list
     int mtiles;       // groups of ROWT * 128 rows a head
     float scale;      // |scale| * log2(e)
     uint32_t flip;    // sign bits of two elements when the scale is negative: the queries take the sign
@@ -57,11 +58,12 @@ struct TreeMmaShape {
     static constexpr int kRing = D == 128 ? (ROWT == 2 ? 5 : 6) : 8;
     static constexpr int kQ = ROWT * 128 * D * 2;
     static constexpr int kExtras = 3072;
+    static constexpr int kUnitCost = 3;  // what a change of units costs, in tiles
     static constexpr int kSmem = kQ + kRing * kBuffer + kExtras;
 };
 
 struct TreeMmaExtras {
-    uint64_t full[8], empty[8], s_ready[2][2], p_ready[2][2], pv_done[2][2], q_ready, done[2];
+    uint64_t full[8], empty[8], s_ready[2][2], p_ready[2][2], pv_done[2][2], q_ready, done;
     int64_t left;
     uint32_t tmem;
     int abort, begin_b, begin_u, begin_j, pad;
@@ -77,10 +79,13 @@ __device__ __forceinline__ int tree_tiles(const TreeArgs &a, int b) {
     return length <= 0 ? 1 : static_cast<int>((length + kTile - 1) / kTile);
 }
 
-// The units that a CTA's range of tiles runs through.
+// The units that a CTA's range of the list runs through.  Every unit is as long as its tiles and COST places that stand for
+// the work of changing units.
+template <int COST>
 struct TreeWalk {
-    int64_t left;
+    int64_t left;  // places still to come
     int b, u, j0, j1, tiles, seg;
+    bool first;  // the range begins inside this unit (its part goes to the CTA's first slot)
     int64_t context, length;
     int used;
     __device__ __forceinline__ void begin(const TreeMmaExtras &x) {
@@ -90,11 +95,27 @@ struct TreeWalk {
         j1 = x.begin_j;
         seg = -1;
         tiles = -1;
+        first = true;
     }
     __device__ __forceinline__ bool next(const TreeArgs &a, int units) {
-        if (left <= 0)
-            return false;
-        if (tiles >= 0 && j1 == tiles) {
+        while (left > 0) {
+            if (tiles < 0) {
+                context = tree_context(a, b);
+                used = tree_used(a, b);
+                length = tree_length(a, b);
+                tiles = length <= 0 ? 1 : static_cast<int>((length + kTile - 1) / kTile);
+            }
+            if (j1 < tiles) {
+                if (seg >= 0)
+                    first = false;
+                j0 = j1;
+                j1 = left < tiles - j0 ? j0 + static_cast<int>(left) : tiles;
+                left -= j1 - j0;
+                seg++;
+                return true;
+            }
+            left -= tiles + COST - j1;  // the places behind the tiles
+            first = false;
             j1 = 0;
             if (++u == units) {
                 u = 0;
@@ -102,17 +123,7 @@ struct TreeWalk {
                 tiles = -1;
             }
         }
-        if (tiles < 0) {
-            context = tree_context(a, b);
-            used = tree_used(a, b);
-            length = tree_length(a, b);
-            tiles = length <= 0 ? 1 : static_cast<int>((length + kTile - 1) / kTile);
-        }
-        j0 = j1;
-        j1 = left < tiles - j0 ? j0 + static_cast<int>(left) : tiles;
-        left -= j1 - j0;
-        seg++;
-        return true;
+        return false;
     }
     __device__ __forceinline__ bool whole() const { return j0 == 0 && j1 == tiles; }
 };
@@ -171,18 +182,20 @@ __device__ __forceinline__ void tree_copy_role(const TreeMmaArgs &g, const CUten
                 }
             }
             fence_proxy_async();
-            mbar_arrive(smem_addr(&x.full[place]));
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(smem_addr(&x.full[place]));
         }
     };
     // the next buffer may be filled; older ones are announced first when that has to be waited for
     auto claim = [&]() {
         const uint32_t bar = smem_addr(&x.empty[next % NB]), parity = ((next / NB) & 1) ^ 1;
-        if (!mbar_try(bar, parity)) {
+        if (!__all_sync(kFullMask, mbar_try(bar, parity))) {
             copy_wait<0>();
             announce(next);
             mbar_wait(bar, parity, abort);
+            __syncwarp();
         }
-        __syncwarp();
     };
     auto issued = [&]() {  // a buffer is a group of copies, a self-announcing one an empty group
         copy_commit();
@@ -197,8 +210,6 @@ __device__ __forceinline__ void tree_copy_role(const TreeMmaArgs &g, const CUten
         const uint32_t bar = smem_addr(&x.full[next % NB]), buf = ring + static_cast<uint32_t>(next % NB) * Shape::kBuffer;
         if (lane == 0)
             mbar_arrive_expect(bar, 32 * D * 2);
-        else
-            mbar_arrive(bar);
         const int row = lane / (D / 64) * g.box_rows;  // this lane's copy: rows from here on, one of the 64-wide column blocks
         const int page_of = __shfl_sync(kFullMask, page, row & 31), slot_of = __shfl_sync(kFullMask, slot, row & 31);
         if (row < 32)
@@ -220,7 +231,7 @@ __device__ __forceinline__ void tree_copy_role(const TreeMmaArgs &g, const CUten
         }
         issued();
     };
-    TreeWalk walk;
+    TreeWalk<Shape::kUnitCost> walk;
     walk.begin(x);
     int tile = 0;
     while (walk.next(a, units)) {
@@ -234,6 +245,8 @@ __device__ __forceinline__ void tree_copy_role(const TreeMmaArgs &g, const CUten
             return j < walk.j1 && pos < walk.length && page < static_cast<uint32_t>(a.max_pages) ? a.table[walk.b * a.table_stride + page] : -1;
         };
         int slot, slot_next = 0, page_next = look(walk.j0, &slot_next);
+        if (walk.seg == 0)
+            asm volatile("bar.sync 2, 384;" ::: "memory");
         for (int j = walk.j0; j < walk.j1; j++, tile++) {
             const int page = page_next;
             slot = slot_next;
@@ -275,87 +288,102 @@ __device__ __forceinline__ void tree_copy_role(const TreeMmaArgs &g, const CUten
         mbar_wait(smem_addr(&x.full[n % NB]), (n / NB) & 1, &gave_up);
 }
 
-// ---- products of softmax group w ----
+// ---- products ----
 template <typename T, int D, int ROWT>
-__device__ __forceinline__ void tree_product_role(const TreeMmaArgs &g, TreeMmaExtras &x, uint32_t q_smem, uint32_t ring, int units, int w) {
+__device__ __forceinline__ void tree_product_role(const TreeMmaArgs &g, TreeMmaExtras &x, uint32_t q_smem, uint32_t ring, int units) {
     using Shape = TreeMmaShape<D, ROWT>;
     constexpr int NB = Shape::kRing;
     constexpr uint32_t qk = mma_instruction<T>(128, kHalf, false), pv = mma_instruction<T>(128, D, true);
+    constexpr int PER = ROWT == 2 ? 2 : 1;  // S tiles of a group in a tile of positions
     volatile int *abort = &x.abort;
     const uint32_t tmem = __shfl_sync(kFullMask, x.tmem, 0);
-    const uint32_t t_s = tmem + w * 2 * kHalf, t_o = tmem + 4 * kHalf + w * D;
-    int made = 0;     // S tiles made
-    int weighed = 0;  // P tiles multiplied
-    int first = 0;    // first buffer of the unit's tiles (keys, values, keys, ...)
+    const uint32_t full = smem_addr(x.full), empty = smem_addr(x.empty), s_ready = smem_addr(x.s_ready), p_ready = smem_addr(x.p_ready),
+                   pv_done = smem_addr(x.pv_done);
+    // the path from the weights to the next S is what the softmax waits for: little is computed on it
+    const uint64_t q_desc = mma_operand(q_smem, 16, 1024), k_desc = mma_operand(ring, 16, 1024), v_desc = mma_operand(ring, kTile * 128, 1024);
+    int step = 0;  // S tiles made for each group
+    uint32_t kn = 0, k_phase = 0, vn = 1, v_phase = 0;  // ring places of the keys and values to be used next, and their phases
     bool ok = true;
-    auto wait = [&](uint64_t &bar, int phase) { ok = __all_sync(kFullMask, mbar_wait(smem_addr(&bar), phase & 1, abort)) && ok; };
-    auto score = [&](int n, int half, bool last) {  // next S = Q K^T from a half of buffer n, which is free after its last use
-        wait(x.full[n % NB], n / NB);
-        const uint32_t to = __shfl_sync(kFullMask, t_s + (made & 1) * kHalf, 0);
-        const uint32_t kb = __shfl_sync(kFullMask, ring + static_cast<uint32_t>(n % NB) * Shape::kBuffer + half * (kHalf * 128), 0);
-        const uint32_t qb = q_smem + (ROWT == 2 ? static_cast<uint32_t>(w) * (128 * D * 2) : 0u);
-        tc_fence_after();
-        if (elect_one()) {
-            if (ok) {
-#pragma unroll
-                for (int k = 0; k < D / 16; k++)
-                    mma_ss(to, mma_operand(qb + (k >> 2) * (128 * 128) + (k & 3) * 32, 16, 1024),
-                           mma_operand(kb + (k >> 2) * (kTile * 128) + (k & 3) * 32, 16, 1024), qk, k > 0);
-            }
-            mma_commit(smem_addr(&x.s_ready[w][made & 1]));
-            if (last)
-                mma_commit(smem_addr(&x.empty[n % NB]));
-        }
-        __syncwarp();
-        made++;
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+        if (!mbar_try(bar, parity))
+            ok = mbar_wait(bar, parity, abort) && ok;
     };
-    auto weigh = [&](int n, int half, bool add, bool last) {  // O += P V from a half of buffer n
-        wait(x.full[n % NB], n / NB);
-        wait(x.p_ready[w][weighed & 1], weighed >> 1);
-        const uint32_t vb = __shfl_sync(kFullMask, ring + static_cast<uint32_t>(n % NB) * Shape::kBuffer + half * (kHalf * 128), 0);
-        const uint32_t from = __shfl_sync(kFullMask, t_s + (weighed & 1) * kHalf, 0);
-        tc_fence_after();
-        if (elect_one()) {
-            if (ok) {
-#pragma unroll
-                for (int k = 0; k < kHalf / 16; k++)
-                    mma_ts(t_o, from + k * 8, mma_operand(vb + k * 2048, kTile * 128, 1024), pv, add || k > 0);
-            }
-            mma_commit(smem_addr(&x.pv_done[w][weighed & 1]));
-            if (last)
-                mma_commit(smem_addr(&x.empty[n % NB]));
+    auto advance = [&](uint32_t &n, uint32_t &phase) {  // keys and values alternate in the ring
+        n += 2;
+        if (n >= NB) {
+            n -= NB;
+            phase ^= 1;
         }
-        __syncwarp();
-        weighed++;
     };
-    TreeWalk walk;
+    TreeWalk<Shape::kUnitCost> walk;
     walk.begin(x);
     while (walk.next(g.a, units)) {
-        constexpr int PER = ROWT == 2 ? 2 : 1;  // S tiles a tile of positions
         const int n = (walk.j1 - walk.j0) * PER;
-        auto half_of = [&](int i) { return ROWT == 2 ? i & 1 : w; };
-        auto last_of = [&](int i) { return ROWT == 1 || (i & 1); };
-        wait(x.q_ready, walk.seg);
-        for (int i = 0; i < 2 && i < n; i++)
-            score(first + i / PER * 2, half_of(i), last_of(i));
-        for (int i = 0; i < n; i++) {
-            weigh(first + i / PER * 2 + 1, half_of(i), i > 0, last_of(i));
-            if (i + 2 < n)
-                score(first + (i + 2) / PER * 2, half_of(i), last_of(i));
+        wait(smem_addr(&x.q_ready), walk.seg & 1);
+        // step i of a group: O += P(i) V, then S(i + 2) in P(i)'s place; steps -2 and -1 make the first two S
+        for (int i = -2; i < n; i++) {
+            const bool weigh = i >= 0, make = i + 2 < n;
+            const bool last = ROWT == 1 || (i & 1);  // of a tile's uses: its buffers are free then
+            if (make && (ROWT == 1 || !(i & 1)))
+                wait(full + kn * 8, k_phase);
+            if (weigh && (ROWT == 1 || !(i & 1)))
+                wait(full + vn * 8, v_phase);
+            // P(i) and S(i + 2) have the same parity; tiles are counted over all units
+            const uint32_t odd = static_cast<uint32_t>(step) & 1, p_phase = static_cast<uint32_t>(step - 2) >> 1 & 1;
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                const uint32_t half = (ROWT == 2 ? i & 1 : w) * (kHalf * 128);
+                const uint64_t qd = q_desc + (ROWT == 2 ? w * (128 * D * 2 / 16) : 0), kd = k_desc + ((kn * Shape::kBuffer + half) >> 4),
+                               vd = v_desc + ((vn * Shape::kBuffer + half) >> 4);
+                const uint32_t at = tmem + w * 2 * kHalf + odd * kHalf;
+                if (weigh)
+                    wait(p_ready + w * 16 + odd * 8, p_phase);
+                __syncwarp();
+                tc_fence_after();
+                if (elect_one()) {
+                    if (weigh) {
+                        if (ok) {
+#pragma unroll
+                            for (int k = 0; k < kHalf / 16; k++)
+                                mma_ts(tmem + 4 * kHalf + w * D, at + k * 8, vd + k * (2048 / 16), pv, i > 0 || k > 0);
+                        }
+                        mma_commit(pv_done + w * 16 + odd * 8);
+                        if (last && w == 1)
+                            mma_commit(empty + vn * 8);
+                    }
+                    if (make) {
+                        if (ok) {
+#pragma unroll
+                            for (int k = 0; k < D / 16; k++)
+                                mma_ss(at, qd + ((k >> 2) * (128 * 128) + (k & 3) * 32) / 16, kd + ((k >> 2) * (kTile * 128) + (k & 3) * 32) / 16, qk, k > 0);
+                        }
+                        mma_commit(s_ready + w * 16 + odd * 8);
+                        if (last && w == 1)
+                            mma_commit(empty + kn * 8);
+                    }
+                }
+                __syncwarp();
+            }
+            if (make && last)
+                advance(kn, k_phase);
+            if (weigh && last)
+                advance(vn, v_phase);
+            step++;
         }
-        first += 2 * (walk.j1 - walk.j0);
+        step -= 2;
     }
     // tensor memory may be given back once nothing writes to it any more
     if (elect_one())
-        mma_commit(smem_addr(&x.done[w]));
+        mma_commit(smem_addr(&x.done));
     __syncwarp();
     volatile int gave_up = 0;
-    mbar_wait(smem_addr(&x.done[w]), 0, &gave_up);
+    mbar_wait(smem_addr(&x.done), 0, &gave_up);
 }
 
 // ---- softmax and output ----
 template <typename T, int D, int ROWT>
 __device__ __forceinline__ void tree_softmax_role(const TreeMmaArgs &g, TreeMmaExtras &x, unsigned char *q_ptr, int units) {
+    using Shape = TreeMmaShape<D, ROWT>;
     const TreeArgs &a = g.a;
     const int tid = threadIdx.x, w = tid >> 7, trow = tid & 127;
     volatile int *abort = &x.abort;
@@ -364,42 +392,50 @@ __device__ __forceinline__ void tree_softmax_role(const TreeMmaArgs &g, TreeMmaE
     int seen = 0;  // S tiles that this group has worked on
     int tile = 0;  // tiles of the units before this one
     bool ok = true;
-    auto wait = [&](uint64_t &bar, int phase) { ok = __all_sync(kFullMask, mbar_wait(smem_addr(&bar), phase & 1, abort)) && ok; };
+    auto wait = [&](uint64_t &bar, int phase) {
+        if (!__all_sync(kFullMask, mbar_try(smem_addr(&bar), phase & 1)))
+            ok = __all_sync(kFullMask, mbar_wait(smem_addr(&bar), phase & 1, abort)) && ok;
+    };
     // a barrier serves every other product: its parity tells a phase from the one before and the one after
     auto wait_weighed = [&](int k) { wait(x.pv_done[w][k & 1], k >> 1); };
-    auto row_of = [&](const TreeWalk &at) { return at.u % g.mtiles * (ROWT * 128) + (ROWT == 2 ? w * 128 : 0) + trow; };
+    auto row_of = [&](const TreeWalk<Shape::kUnitCost> &at) { return at.u % g.mtiles * (ROWT * 128) + (ROWT == 2 ? w * 128 : 0) + trow; };
     // queries and parents of a unit into shared memory
-    auto load_unit = [&](const TreeWalk &at) {
+    auto load_unit = [&](const TreeWalk<Shape::kUnitCost> &at, bool first) {
         if (static_cast<int64_t>(at.j1) * kTile > at.context && trow < a.nodes) {
             const int up = a.parents ? a.parents[static_cast<int64_t>(at.b) * a.nodes + trow] : trow - 1;
             x.parents[w][trow] = up >= 0 && up < trow ? up : 255;
         }
-        constexpr int PIECES = ROWT == 2 ? D / 8 : D / 16;
-        const int from = ROWT == 2 ? 0 : w * PIECES, row = row_of(at), node = row / a.group;
-        const bool live = row < a.rows && node < at.used;
-        const T *src = static_cast<const T *>(a.q) + at.b * a.q_bs + node * a.q_ns + (at.u / g.mtiles * a.group + row % a.group) * a.q_hs;
-        unsigned char *dst = q_ptr + (ROWT == 2 ? w * (128 * D * 2) : 0) + trow * 128;
-        uint4 q[PIECES];  // all loads first: the stores below would hold the next load back
+        // a warp loads whole rows, two (four) at a time, all loads before the stores
+        constexpr int PIECES = D / 8, TOGETHER = 32 / PIECES, ROWS = ROWT == 2 ? 32 : 16, LOADS = ROWS / TOGETHER;
+        const int lane = tid & 31, piece = lane % PIECES, r0 = (tid >> 5) * ROWS + lane / PIECES;
+        const int base = at.u % g.mtiles * (ROWT * 128), h = at.u / g.mtiles;
+        uint4 q[LOADS];
 #pragma unroll
-        for (int c = 0; c < PIECES; c++)
-            q[c] = live ? *reinterpret_cast<const uint4 *>(src + (from + c) * 8) : make_uint4(0, 0, 0, 0);
+        for (int c = 0; c < LOADS; c++) {
+            const int row = base + r0 + c * TOGETHER, node = row / a.group;
+            q[c] = make_uint4(0, 0, 0, 0);
+            if (row < a.rows && node < at.used)
+                q[c] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + at.b * a.q_bs + node * a.q_ns + (h * a.group + row - node * a.group) * a.q_hs + piece * 8);
+        }
+        if (first)  // the copies wait for this: the first queries would otherwise queue behind all of the first keys and values
+            asm volatile("bar.arrive 2, 384;" ::: "memory");
 #pragma unroll
-        for (int c = 0; c < PIECES; c++) {
-            const int piece = from + c;
+        for (int c = 0; c < LOADS; c++) {
+            const int r = r0 + c * TOGETHER;
             uint4 v = q[c];
             v.x = (v.x ^ g.flip) & g.mask, v.y = (v.y ^ g.flip) & g.mask, v.z = (v.z ^ g.flip) & g.mask, v.w = (v.w ^ g.flip) & g.mask;
-            *reinterpret_cast<uint4 *>(dst + (piece >> 3) * (128 * 128) + (((piece & 7) ^ (trow & 7)) << 4)) = v;
+            *reinterpret_cast<uint4 *>(q_ptr + (r >> 7) * (128 * D * 2) + (r & 127) * 128 + (piece >> 3) * (128 * 128) + (((piece & 7) ^ (r & 7)) << 4)) = v;
         }
         fence_proxy_async();
         mbar_arrive(smem_addr(&x.q_ready));
     };
-    TreeWalk ahead;
+    TreeWalk<Shape::kUnitCost> ahead;
     ahead.begin(x);
     bool more = ahead.next(a, units);
     if (more)
-        load_unit(ahead);
+        load_unit(ahead, true);
     while (more) {
-        const TreeWalk walk = ahead;
+        const TreeWalk<Shape::kUnitCost> walk = ahead;
         const int b = walk.b, h = walk.u / g.mtiles, n = walk.j1 - walk.j0, row = row_of(walk);
         const bool row_ok = row < a.rows;
         const int node = row_ok ? row / a.group : 0, head = h * a.group + (row_ok ? row % a.group : 0);
@@ -503,7 +539,9 @@ __device__ __forceinline__ void tree_softmax_role(const TreeMmaArgs &g, TreeMmaE
                 tmem_wait_store();
             }
             tc_fence_before();
-            mbar_arrive(smem_addr(&x.p_ready[w][seen & 1]));
+            __syncwarp();
+            if ((tid & 31) == 0)
+                mbar_arrive(smem_addr(&x.p_ready[w][seen & 1]));
         }
         // ---- the unit's rows, or this CTA's part of them ----
         // a padding node's row took part with zeros where the tile was not masked: it attends nothing
@@ -527,7 +565,7 @@ __device__ __forceinline__ void tree_softmax_role(const TreeMmaArgs &g, TreeMmaE
         }
         more = ahead.next(a, units);
         if (more)
-            load_unit(ahead);
+            load_unit(ahead, false);
         if (seen > 1)
             wait_weighed(seen - 2);
         wait_weighed(seen - 1);
@@ -537,13 +575,14 @@ __device__ __forceinline__ void tree_softmax_role(const TreeMmaArgs &g, TreeMmaE
         }
         tc_fence_after();
         const bool whole = walk.whole();
-        const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + (walk.seg > 0)) * (ROWT * 128) + (ROWT == 2 ? w * 128 : 0) + trow;
+        const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + !walk.first;
+        const int part_row = (ROWT == 2 ? w * 128 : 0) + trow;
         T *o_row = static_cast<T *>(a.out) + b * a.o_bs + node * a.o_ns + head * a.o_hs;
         const bool empty = l == 0.0f;
         const float inv = empty ? 0.0f : 1.0f / l;
         const bool broken = *reinterpret_cast<volatile int *>(&x.bad[walk.seg & (kSlots - 1)]) != 0;
         if (__any_sync(kFullMask, row_ok)) {
-#pragma unroll
+#pragma unroll 1  // code that runs once a unit: its fetch is what it costs
             for (int c = 0; c < COLS / 32; c++) {
                 const int col = (ROWT == 2 ? 0 : w * COLS) + 32 * c;
                 uint32_t o[32];
@@ -610,17 +649,16 @@ __device__ __forceinline__ void tree_softmax_role(const TreeMmaArgs &g, TreeMmaE
                         }
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8)  // whole sectors
-                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(a.part_o + slot * D + col + i), "r"(o[i]),
-                                         "r"(o[i + 1]), "r"(o[i + 2]), "r"(o[i + 3]), "r"(o[i + 4]), "r"(o[i + 5]), "r"(o[i + 6]), "r"(o[i + 7])
-                                         : "memory");
+                        for (int i = 0; i < 32; i += 4)  // [column / 4][row][4]: the lanes' stores are neighbours
+                            *reinterpret_cast<uint4 *>(a.part_o + ((slot * (D / 4) + (col + i) / 4) * (ROWT * 128) + part_row) * 4) =
+                                make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                     }
                 }
                 __syncwarp();
             }
             if (row_ok && (ROWT == 2 || w == 0)) {
                 if (!whole)
-                    a.part_ml[slot] = make_float2(m, l);
+                    a.part_ml[slot * (ROWT * 128) + part_row] = make_float2(m, l);
                 else if (a.lse)
                     a.lse[(static_cast<int64_t>(b) * a.nodes + node) * a.q_heads + head] = empty ? -INFINITY : (m + log2f(l)) * kLn2;
             }
@@ -641,6 +679,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_attention_mma_kernel(cons
     const TreeArgs &a = g.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int units = a.kv_heads * g.mtiles;
+    auto places = [&](int tiles) { return static_cast<int64_t>(tiles + Shape::kUnitCost) * units; };
 
     // this CTA's range of the list of all tiles
     int64_t *s_scan = reinterpret_cast<int64_t *>(smem);
@@ -651,7 +690,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_attention_mma_kernel(cons
     for (int b = b0; b < b1; b++) {
         const int tiles = tree_tiles(a, b);
         tiles0 = b == b0 ? tiles : tiles0;
-        sum += static_cast<int64_t>(tiles) * units;
+        sum += places(tiles);
     }
     int64_t upto = sum;
 #pragma unroll
@@ -663,18 +702,18 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_attention_mma_kernel(cons
         s_scan[warp] = upto;
     if (tid == 0) {
         for (int i = 0; i < 8; i++) {
-            mbar_init(smem_addr(&x.full[i]), 128);
-            mbar_init(smem_addr(&x.empty[i]), 2);
+            mbar_init(smem_addr(&x.full[i]), 4);   // a copy warp each
+            mbar_init(smem_addr(&x.empty[i]), 1);
         }
         for (int i = 0; i < 2; i++) {
-            mbar_init(smem_addr(&x.done[i]), 1);
             for (int k = 0; k < 2; k++) {
                 mbar_init(smem_addr(&x.s_ready[i][k]), 1);
-                mbar_init(smem_addr(&x.p_ready[i][k]), 128);
+                mbar_init(smem_addr(&x.p_ready[i][k]), 4);  // a softmax warp each
                 mbar_init(smem_addr(&x.pv_done[i][k]), 1);
             }
         }
         mbar_init(smem_addr(&x.q_ready), 256);
+        mbar_init(smem_addr(&x.done), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         x.abort = 0;
         x.left = 0;
@@ -687,12 +726,12 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_attention_mma_kernel(cons
         before += i < warp ? s_scan[i] : 0;
         total += s_scan[i];
     }
-    const int64_t lo = blockIdx.x * total / gridDim.x, hi = (blockIdx.x + 1) * total / gridDim.x;
+    const int64_t lo = blockIdx.x * total / kMmaCtas, hi = (blockIdx.x + 1) * total / kMmaCtas;
     if (blockIdx.x == 0) {
         int64_t at = before;
         for (int b = b0; b < b1; b++) {
             g.starts[b] = at;
-            at += static_cast<int64_t>(b == b0 ? tiles0 : tree_tiles(a, b)) * units;
+            at += places(b == b0 ? tiles0 : tree_tiles(a, b));
         }
         if (tid == 0)
             g.starts[a.batch] = total;
@@ -700,13 +739,15 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_attention_mma_kernel(cons
     if (lo < hi && lo >= before && lo < before + sum) {
         int64_t at = before;
         int b = b0, tiles = tiles0;
-        while (lo >= at + static_cast<int64_t>(tiles) * units) {
-            at += static_cast<int64_t>(tiles) * units;
+        while (lo >= at + places(tiles)) {
+            at += places(tiles);
             tiles = tree_tiles(a, ++b);
         }
         x.begin_b = b;
-        x.begin_u = static_cast<int>((lo - at) / tiles);
-        x.begin_j = static_cast<int>((lo - at) % tiles);
+        const int one = tiles + Shape::kUnitCost;
+        const int64_t into = lo - at;
+        x.begin_u = into >> 32 ? static_cast<int>(into / one) : static_cast<int>(static_cast<uint32_t>(into) / static_cast<uint32_t>(one));
+        x.begin_j = static_cast<int>(into - static_cast<int64_t>(x.begin_u) * one);
         x.left = hi - lo;
     }
     if (lo >= hi)
@@ -722,8 +763,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_attention_mma_kernel(cons
         tree_softmax_role<T, D, ROWT>(g, x, smem, units);
     else if (warp < 12)
         tree_copy_role<T, D, ROWT>(g, &k_map, &v_map, x, ring, units);
-    else if (warp < 14)
-        tree_product_role<T, D, ROWT>(g, x, q_smem, ring, units, warp - 12);
+    else if (warp == 12)
+        tree_product_role<T, D, ROWT>(g, x, q_smem, ring, units);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -731,66 +772,83 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_attention_mma_kernel(cons
         tmem_free(x.tmem, 512);
 }
 
-// ---- join: one warp a row of a unit that several CTAs worked on ----
-constexpr int kMmaJoinWarps = 8;
+// ---- join: a unit that several CTAs worked on; a thread takes a row's D / 8 neighbouring columns, so that a warp reads the
+// parts of 32 rows as they lie; parts are added in the order of the CTAs ----
+constexpr int kMmaJoinRows = 32;
 
 template <typename T, int D, int ROWT>
-__global__ void __launch_bounds__(kMmaJoinWarps * 32) tree_attention_mma_join_kernel(const TreeMmaArgs g, int ctas) {
+__global__ void __launch_bounds__(kMmaJoinRows * 8) tree_attention_mma_join_kernel(const TreeMmaArgs g) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    constexpr int COLS = D / 8;
     const TreeArgs &a = g.a;
-    const int lane = threadIdx.x & 31, units = a.kv_heads * g.mtiles;
-    const int b = blockIdx.x / units, u = blockIdx.x % units;
-    const int in_unit = blockIdx.y * kMmaJoinWarps + (threadIdx.x >> 5), row = u % g.mtiles * (ROWT * 128) + in_unit;
-    if (row >= a.rows)
-        return;
-    const int64_t total = g.starts[a.batch], first = g.starts[b], tiles = (g.starts[b + 1] - first) / units;
-    const int64_t lo = first + u * tiles, hi = lo + tiles;
-    const int c0 = static_cast<int>(((lo + 1) * ctas - 1) / total), c1 = static_cast<int>((hi * ctas - 1) / total);
+    const int units = a.kv_heads * g.mtiles, b = blockIdx.x / units, u = blockIdx.x % units;
+    const int in_unit = blockIdx.y * kMmaJoinRows + (threadIdx.x & 31), col = (threadIdx.x >> 5) * COLS;
+    const int row = u % g.mtiles * (ROWT * 128) + in_unit;
+    const int64_t total = g.starts[a.batch], begin = g.starts[b], places = (g.starts[b + 1] - begin) / units;
+    const int64_t lo = begin + u * places, hi = lo + places - TreeMmaShape<D, ROWT>::kUnitCost;  // the unit's tiles
+    const int c0 = static_cast<int>(((lo + 1) * kMmaCtas - 1) / total), c1 = static_cast<int>((hi * kMmaCtas - 1) / total);
     if (c0 == c1)
         return;  // written out by the one CTA
-    // CTA c's part lies in its first slot when its range begins inside the unit, else in its second; a range may be empty.
-    // The lanes look 32 parts up at a time; parts are added in the order of the CTAs.
-    float top = -INFINITY, l = 0.0f, acc[D / 32];
+    float top = -INFINITY, l = 0.0f, acc[COLS];
 #pragma unroll
-    for (int e = 0; e < D / 32; e++)
+    for (int e = 0; e < COLS; e++)
         acc[e] = 0.0f;
-    for (int c = c0; c <= c1; c += 32) {
-        const int mine = c + lane;
-        int slot = -1;
-        float2 ml = make_float2(-INFINITY, 0.0f);
-        if (mine <= c1) {
-            const int64_t from = mine * total / ctas;
-            if (from != (mine + 1) * total / ctas) {
-                slot = (mine * 2 + (from < lo)) * (ROWT * 128) + in_unit;
-                ml = a.part_ml[slot];
+    __shared__ int s_slot[32];
+    __shared__ float2 s_ml[32][kMmaJoinRows];
+    const int lane = threadIdx.x & 31;
+    for (int c = c0; c <= c1; c += 32) {  // 32 parts at a time
+        const int count = min(32, c1 - c + 1);
+        if (static_cast<int>(threadIdx.x) < count) {
+            const int64_t at = c + threadIdx.x, from = at * total / kMmaCtas;
+            // the CTA's first slot when its range begins inside the unit; an empty range has none
+            s_slot[threadIdx.x] = from == (at + 1) * total / kMmaCtas ? -1 : static_cast<int>(at * 2 + (from < lo));
+        }
+        __syncthreads();
+        for (int p = threadIdx.x >> 5; p < count; p += 8)
+            s_ml[p][lane] = s_slot[p] >= 0 && row < a.rows ? a.part_ml[static_cast<int64_t>(s_slot[p]) * (ROWT * 128) + in_unit] : make_float2(-INFINITY, 0.0f);
+        __syncthreads();
+        float higher = top;
+        for (int p = 0; p < count; p++)
+            higher = fmaxf(higher, s_ml[p][lane].x);
+        const float base = higher == -INFINITY ? 0.0f : higher, keep = exp2_approx(top - base);
+        top = higher;
+        l *= keep;
+#pragma unroll
+        for (int e = 0; e < COLS; e++)
+            acc[e] *= keep;
+#pragma unroll 2
+        for (int p = 0; p < count; p++) {
+            const int slot = s_slot[p];
+            if (slot < 0 || row >= a.rows)
+                continue;
+            const float4 *o = reinterpret_cast<const float4 *>(a.part_o) + (static_cast<int64_t>(slot) * (D / 4) + col / 4) * (ROWT * 128) + in_unit;
+            const float f = exp2_approx(s_ml[p][lane].x - base);
+            l = fmaf(f, s_ml[p][lane].y, l);
+#pragma unroll
+            for (int e = 0; e < COLS / 4; e++) {
+                const float4 v = o[e * (ROWT * 128)];
+                acc[4 * e] = fmaf(f, v.x, acc[4 * e]);
+                acc[4 * e + 1] = fmaf(f, v.y, acc[4 * e + 1]);
+                acc[4 * e + 2] = fmaf(f, v.z, acc[4 * e + 2]);
+                acc[4 * e + 3] = fmaf(f, v.w, acc[4 * e + 3]);
             }
         }
-        const float higher = fmaxf(top, warp_max(ml.x)), base = higher == -INFINITY ? 0.0f : higher, keep = exp2f(top - base);
-        const float f = exp2f(ml.x - base);
-        top = higher;
-        l = l * keep + warp_sum(f * ml.y);
-#pragma unroll
-        for (int e = 0; e < D / 32; e++)
-            acc[e] *= keep;
-        const int count = min(32, c1 - c + 1);
-#pragma unroll 8
-        for (int p = 0; p < count; p++) {
-            const int at = __shfl_sync(kFullMask, slot, p);
-            const float w = __shfl_sync(kFullMask, f, p);
-            if (at < 0)
-                continue;
-#pragma unroll
-            for (int e = 0; e < D / 32; e++)
-                acc[e] = fmaf(w, a.part_o[static_cast<int64_t>(at) * D + lane + 32 * e], acc[e]);
-        }
+        __syncthreads();
     }
+    if (row >= a.rows)
+        return;
     const int node = row / a.group, head = u / g.mtiles * a.group + row % a.group;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    T *o = static_cast<T *>(a.out) + b * a.o_bs + node * a.o_ns + head * a.o_hs;
+    T *out = static_cast<T *>(a.out) + b * a.o_bs + node * a.o_ns + head * a.o_hs + col;
 #pragma unroll
-    for (int e = 0; e < D / 32; e++)
-        o[lane + 32 * e] = Elem<T>::to_storage(l == 0.0f ? 0.0f : acc[e] * inv);
-    if (a.lse && lane == 0)
+    for (int e = 0; e < COLS; e += 8) {
+        uint32_t v[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            v[k] = l == 0.0f ? 0u : TcType<T>::pack(acc[e + 2 * k] * inv, acc[e + 2 * k + 1] * inv);
+        *reinterpret_cast<uint4 *>(out + e) = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+    if (a.lse && col == 0)
         a.lse[(static_cast<int64_t>(b) * a.nodes + node) * a.q_heads + head] = l == 0.0f ? -INFINITY : (top + log2f(l)) * kLn2;
 }
 
@@ -820,15 +878,15 @@ static int launch_mma_t(const TreeMmaArgs &g, const CUtensorMap *maps, cudaStrea
         return VKOP_CUDA_ERROR;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(g.a.batch * g.a.kv_heads * g.mtiles),
-                       static_cast<unsigned>((min(g.a.rows, ROWT * 128) + kMmaJoinWarps - 1) / kMmaJoinWarps));
-    cfg.blockDim = dim3(kMmaJoinWarps * 32);
+                       static_cast<unsigned>((min(g.a.rows, ROWT * 128) + kMmaJoinRows - 1) / kMmaJoinRows));
+    cfg.blockDim = dim3(kMmaJoinRows * 8);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, tree_attention_mma_join_kernel<T, D, ROWT>, g, kMmaCtas) != cudaSuccess) {
+    if (cudaLaunchKernelEx(&cfg, tree_attention_mma_join_kernel<T, D, ROWT>, g) != cudaSuccess) {
         cudaGetLastError();
         return VKOP_CUDA_ERROR;
     }
@@ -870,7 +928,7 @@ static bool cache_map(CUtensorMap *map, int dtype, const void *base, int64_t num
 int launch_tree_mma(const TreeArgs &args, int dtype, void *workspace, cudaStream_t stream) {
     TreeMmaArgs g;
     g.a = args;
-    workspace = reinterpret_cast<void *>((reinterpret_cast<uintptr_t>(workspace) + 31) / 32 * 32);  // the parts are stored 32 bytes at a time
+    workspace = reinterpret_cast<void *>((reinterpret_cast<uintptr_t>(workspace) + 31) / 32 * 32);
     g.starts = static_cast<int64_t *>(workspace);
     const size_t starts = (static_cast<size_t>(args.batch + 1) * 8 + 31) / 32 * 32;
     g.a.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + starts);
