@@ -278,30 +278,56 @@ def sample_topk(values: torch.Tensor, indices: torch.Tensor, top_p: float, u: to
     return choice, token
 
 
-def _one_device(what: str, *tensors) -> torch.device:
-    """The device that all the tensors lie on (None among them is passed over)."""
-    device = tensors[0].device
+# The bindings below are on the path of every decoding step: checks and bookkeeping are kept to a few microseconds.
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _one_device(what: str, *tensors) -> int:
+    """The index of the device that all the tensors lie on (None among them is passed over)."""
+    index = tensors[0].get_device()
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.device != device):
+        if t is not None and (not t.is_cuda or t.get_device() != index):
             raise RuntimeError(f"{what}: vkop_b200 runs on CUDA device memory only, all tensors on one device")
-    return device
+    return index
+
+
+def _call(index: int, what: str, fn, *args) -> None:
+    """Calls a C entry point with the device current and its current stream as the last argument."""
+    if torch.cuda.current_device() == index:
+        status = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, _raw_stream(index))
+    if status != OK:
+        raise VkopError(status, what)
 
 
 def _whole(what: str, name: str, t, shape, dtype=torch.int32):
     """Checks a small dense argument: its type, its shape and that it is contiguous."""
-    if t is not None and (t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous()):
+    if t is not None and (t.dtype != dtype or t.shape != shape or not t.is_contiguous()):
         raise ValueError(f"{what}: {name} is a contiguous {dtype} tensor of shape {tuple(shape)}, "
                          f"got {t.dtype} {tuple(t.shape)}")
 
 
 def _strides(what: str, name: str, t: torch.Tensor, ndim: int):
-    """Strides of the leading dimensions, in elements; the last dimension is contiguous and nothing is broadcast."""
+    """Strides of the leading dimensions, in elements (0: dense); the last dimension is contiguous and nothing is broadcast."""
     if t.dim() != ndim or t.dtype not in _TORCH_DTYPE:
         raise ValueError(f"{what}: {name} is a float32, float16 or bfloat16 tensor of {ndim} dimensions")
+    if t.is_contiguous():
+        return (0,) * (ndim - 1)
     strides, shape = t.stride(), t.shape
     if (strides[-1] != 1 and shape[-1] > 1) or any(s == 0 and n > 1 for s, n in zip(strides, shape)):
         raise ValueError(f"{what}: {name} has a contiguous last dimension and no broadcast one")
     return [s if n > 1 else 0 for s, n in zip(strides[:-1], shape[:-1])]
+
+
+def _table(what: str, t: torch.Tensor, batch: int) -> int:
+    """Checks a page table; returns the stride of its rows (0: dense)."""
+    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != batch or \
+            not (t.is_contiguous() or (t.stride(1) == 1 and t.stride(0) >= t.shape[1])):
+        raise ValueError(f"{what}: page_table is int32 [batch, max_pages]")
+    return t.stride(0) if batch > 1 else 0
 
 
 def draft_verify(target: torch.Tensor, tokens: torch.Tensor, u: torch.Tensor, draft: torch.Tensor | None = None,
@@ -314,10 +340,10 @@ def draft_verify(target: torch.Tensor, tokens: torch.Tensor, u: torch.Tensor, dr
     parents int32 [batch, nodes]; num_nodes int32 [batch].
     Returns (path int32 [batch, nodes], count int32 [batch], token [batch]), and chance float32 [batch, nodes] if asked."""
     what = "draft_verify"
-    device = _one_device(what, target, tokens, u, draft, parents, num_nodes)
+    index = _one_device(what, target, tokens, u, draft, parents, num_nodes)
     ts = _strides(what, "target", target, 3)
     batch, nodes, vocab = target.shape
-    ds, rows = [0, 0], 0
+    ds, rows = (0, 0), 0
     if draft is not None:
         ds, rows = _strides(what, "draft", draft, 3), draft.shape[1]
         if draft.dtype != target.dtype or draft.shape[0] != batch or draft.shape[2] != vocab:
@@ -330,14 +356,11 @@ def draft_verify(target: torch.Tensor, tokens: torch.Tensor, u: torch.Tensor, dr
     _whole(what, "num_nodes", num_nodes, (batch,))
     desc = DraftVerifyDesc(batch, vocab, ts[0], ts[1], ds[0], ds[1], nodes, rows, dtype_tag(target),
                            I64 if tokens.dtype == torch.int64 else I32)
-    path = torch.empty((batch, nodes), dtype=torch.int32, device=device)
-    count = torch.empty(batch, dtype=torch.int32, device=device)
-    token = torch.empty(batch, dtype=tokens.dtype, device=device)
-    chance = torch.empty((batch, nodes), dtype=torch.float32, device=device) if chances else None
-    with torch.cuda.device(device):
-        check(lib().vkop_cuda_draft_verify(C.byref(desc), target.data_ptr(), _ptr(draft), tokens.data_ptr(), _ptr(parents),
-                                           _ptr(num_nodes), u.data_ptr(), path.data_ptr(), count.data_ptr(),
-                                           token.data_ptr(), _ptr(chance), _stream()), what)
+    path, token = torch.empty_like(tokens, dtype=torch.int32), tokens.new_empty(batch)
+    count = path.new_empty(batch)
+    chance = torch.empty_like(u) if chances else None
+    _call(index, what, lib().vkop_cuda_draft_verify, C.byref(desc), target.data_ptr(), _ptr(draft), tokens.data_ptr(), _ptr(parents),
+          _ptr(num_nodes), u.data_ptr(), path.data_ptr(), count.data_ptr(), token.data_ptr(), _ptr(chance))
     return (path, count, token, chance) if chances else (path, count, token)
 
 
@@ -345,17 +368,14 @@ def _tree_attention_desc(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
                          scale: float | None, max_context: int, out: torch.Tensor | None) -> TreeAttentionDesc:
     what = "tree_attention"
     qs, ks, vs = _strides(what, "q", q, 4), _strides(what, "k_cache", k_cache, 4), _strides(what, "v_cache", v_cache, 4)
-    os_ = _strides(what, "out", out, 4) if out is not None else [0, 0, 0]
+    os_ = _strides(what, "out", out, 4) if out is not None else (0, 0, 0)
     batch, nodes, heads, dim = q.shape
     pages, page_size, kv_heads, kv_dim = k_cache.shape
     if k_cache.shape != v_cache.shape or kv_dim != dim or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
         raise ValueError("tree_attention: k_cache and v_cache are [pages, page_size, kv_heads, head_dim] of q's type and head_dim")
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch or \
-            (page_table.shape[1] > 1 and page_table.stride(1) != 1) or (batch > 1 and page_table.stride(0) < page_table.shape[1]):
-        raise ValueError("tree_attention: page_table is int32 [batch, max_pages]")
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype):
         raise ValueError("tree_attention: out has the shape and type of q")
-    return TreeAttentionDesc(batch, pages, max_context, *qs, *os_, *ks, *vs, page_table.stride(0) if batch > 1 else 0, nodes,
+    return TreeAttentionDesc(batch, pages, max_context, *qs, *os_, *ks, *vs, _table(what, page_table, batch), nodes,
                              heads, kv_heads, dim, page_size, page_table.shape[1], dtype_tag(q),
                              dim ** -0.5 if scale is None else scale)
 
@@ -381,26 +401,24 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     uint8 tensor of tree_attention_workspace_bytes() to use instead of torch's allocator.
     Returns out like q, and lse float32 [batch, nodes, q_heads] if asked."""
     what = "tree_attention"
-    device = _one_device(what, q, k_cache, v_cache, page_table, context, parents, num_nodes, workspace, out)
+    index = _one_device(what, q, k_cache, v_cache, page_table, context, parents, num_nodes, workspace, out)
     desc = _tree_attention_desc(q, k_cache, v_cache, page_table, scale, max_context, out)
     batch, nodes, heads = desc.batch, desc.nodes, desc.q_heads
     _whole(what, "context", context, (batch,))
     _whole(what, "parents", parents, (batch, nodes))
     _whole(what, "num_nodes", num_nodes, (batch,))
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
-    lse = torch.empty((batch, nodes, heads), dtype=torch.float32, device=device) if return_lse else None
-    L = lib()
-    with torch.cuda.device(device):
-        if workspace is None:
-            need = C.c_size_t(0)
-            check(L.vkop_cuda_tree_attention_workspace(C.byref(desc), C.byref(need)), what)
-            if need.value:
-                workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
-        nbytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-        check(L.vkop_cuda_tree_attention(C.byref(desc), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-                                         page_table.data_ptr(), context.data_ptr(), _ptr(parents), _ptr(num_nodes),
-                                         out.data_ptr(), _ptr(lse), _ptr(workspace), nbytes, _stream()), what)
+        out = q.new_empty(q.shape)
+    lse = q.new_empty((batch, nodes, heads), dtype=torch.float32) if return_lse else None
+    L, ref = lib(), C.byref(desc)
+    if workspace is None:
+        need = C.c_size_t(0)
+        check(L.vkop_cuda_tree_attention_workspace(ref, C.byref(need)), what)
+        if need.value:
+            workspace = q.new_empty(need.value, dtype=torch.uint8)
+    nbytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    _call(index, what, L.vkop_cuda_tree_attention, ref, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(),
+          context.data_ptr(), _ptr(parents), _ptr(num_nodes), out.data_ptr(), _ptr(lse), _ptr(workspace), nbytes)
     return (out, lse) if return_lse else out
 
 
@@ -410,11 +428,11 @@ def cache_compact(k_cache: torch.Tensor, v_cache: torch.Tensor | None, page_tabl
     place.  k_cache, v_cache [layers, pages, page_size, kv_heads, head_dim], or without the first dimension for one layer.
     Returns the new context lengths, int32 [batch]."""
     what = "cache_compact"
-    device = _one_device(what, k_cache, v_cache, page_table, context, path, count)
+    index = _one_device(what, k_cache, v_cache, page_table, context, path, count)
     if k_cache.dim() == 4:
         k_cache, v_cache = k_cache[None], v_cache[None] if v_cache is not None else None
     ks = _strides(what, "k_cache", k_cache, 5)
-    vs = _strides(what, "v_cache", v_cache, 5) if v_cache is not None else [0] * 4
+    vs = _strides(what, "v_cache", v_cache, 5) if v_cache is not None else (0, 0, 0, 0)
     if v_cache is not None and (v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype):
         raise ValueError("cache_compact: k_cache and v_cache have one shape and type")
     layers, pages, page_size, heads, dim = k_cache.shape
@@ -425,16 +443,11 @@ def cache_compact(k_cache: torch.Tensor, v_cache: torch.Tensor | None, page_tabl
     _whole(what, "context", context, (batch,))
     _whole(what, "path", path, (batch, nodes))
     _whole(what, "count", count, (batch,))
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch or \
-            (page_table.shape[1] > 1 and page_table.stride(1) != 1) or (batch > 1 and page_table.stride(0) < page_table.shape[1]):
-        raise ValueError("cache_compact: page_table is int32 [batch, max_pages]")
-    desc = CacheCompactDesc(batch, pages, *ks, *vs, page_table.stride(0) if batch > 1 else 0, layers, nodes, heads, dim,
+    desc = CacheCompactDesc(batch, pages, *ks, *vs, _table(what, page_table, batch), layers, nodes, heads, dim,
                             page_size, page_table.shape[1], dtype_tag(k_cache), 0)
-    lengths = torch.empty(batch, dtype=torch.int32, device=device)
-    with torch.cuda.device(device):
-        check(lib().vkop_cuda_cache_compact(C.byref(desc), k_cache.data_ptr(), _ptr(v_cache), page_table.data_ptr(),
-                                            context.data_ptr(), path.data_ptr(), count.data_ptr(), lengths.data_ptr(),
-                                            _stream()), what)
+    lengths = torch.empty_like(context)
+    _call(index, what, lib().vkop_cuda_cache_compact, C.byref(desc), k_cache.data_ptr(), _ptr(v_cache), page_table.data_ptr(),
+          context.data_ptr(), path.data_ptr(), count.data_ptr(), lengths.data_ptr())
     return lengths
 
 
