@@ -103,7 +103,7 @@ def test_ends_of_the_uniform_range_and_degenerate_rows(capi):
     p[1, 0, 5] = p[1, 0, 3999] = 0.5
     p[2, 0] = 0.0                            # nothing to draw
     p[3, 0] = torch.tensor(float("nan"))     # not numbers: nothing either
-    p[4, 0, :4] = torch.tensor([float("inf"), -1.0, float("nan"), 0.25])
+    p[4, 0, :6] = torch.tensor([float("inf"), -1.0, float("nan"), 0.25, 1e-40, -0.0])
     tokens = torch.tensor([[0, 1234], [0, 17], [0, 0], [0, 0], [0, 0]], dtype=torch.int64)
     for first in (0.0, 0.49999, 0.5, 1 - 2.0**-24):
         u = torch.tensor([[first, 0.0]] * 5)

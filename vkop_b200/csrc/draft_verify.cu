@@ -8,8 +8,9 @@
 //          several rejections never has to be written down: max(max(p - c q, 0) / D - q, 0) = max(p - (c + D) q, 0) / D, so
 //          one number c and the mass D describe it.
 //  mass    Only where a second child of a node is tested after a rejection, D = sum max(p - c q, 0) takes a pass over the
-//          vocabulary, and the last token takes one: every warp of the cluster sums a contiguous range of the row, the
-//          sums are read through distributed shared memory and added in one fixed order by everybody.
+//          vocabulary, and the last token takes one: every warp of the cluster sums a contiguous range of the row and stores
+//          its sum into the shared memory of every CTA of the cluster, where one scan in a fixed order gives everybody the
+//          total and the prefixes.
 //  draw    The range in which the prefix sum passes u times the total is read once more (from L2) by the CTA that owns
 //          it: each thread sums a short run, a scan finds the run, its thread walks it.
 //
@@ -17,8 +18,6 @@
 // that of any other 64-bit evaluation only where a random number lies within about 1e-15 of a border.
 // Bound: the one row of p (and of q) per sequence that has to be read, and for few sequences the latency of the chain
 // gather -> walk -> pass -> draw.
-#include <cfloat>
-
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -31,7 +30,6 @@ namespace cg = cooperative_groups;
 constexpr int kVerifyThreads = 512;
 constexpr int kVerifyWarps = kVerifyThreads / 32;
 constexpr int kVerifyMaxCluster = 8;  // portable cluster size
-constexpr int kExcludeBuckets = 8192;  // hash of 8-element groups that hold a rejected token (certain drafts)
 
 struct VerifyArgs {
     const void *target, *draft, *tokens;
@@ -44,12 +42,18 @@ struct VerifyArgs {
     int nodes, draft_rows, index_dtype;
 };
 
-// negative, NaN and infinite entries count as zero
-__device__ __forceinline__ float clean_prob(float v) { return (v > 0.0f && v <= FLT_MAX) ? v : 0.0f; }
+// An entry in 64 bits; negative, NaN and infinite ones, and those below the smallest normal 32-bit number, count as zero.
+// Exact, and put together from the bits: the conversion instruction runs at an eighth of the rate of these operations and
+// took a third of a pass.
+__device__ __forceinline__ double prob64(float v) {
+    const uint32_t u = __float_as_uint(v);
+    const bool good = u - 0x00800000u < 0x7F000000u;
+    return __hiloint2double(good ? static_cast<int>((u >> 3) + 0x38000000u) : 0, good ? static_cast<int>(u << 29) : 0);
+}
 
 template <typename T>
-__device__ __forceinline__ float load_prob(const T *p) {
-    return clean_prob(Elem<T>::from_storage(*p));
+__device__ __forceinline__ double load_prob(const T *p) {
+    return prob64(Elem<T>::from_storage(*p));
 }
 
 // What is summed over a row: p, max(p - c q, 0), or p without the rejected tokens.
@@ -60,23 +64,18 @@ struct RowMass {
     const T *p, *q;
     double c;
     VerifyMass mode;
-    // rejected tokens (kMassExcluded): children of `cur` below `until`
-    const int *par, *tok;
-    const uint32_t *buckets;
-    int cur, until;
+    const int *gone;  // rejected tokens (kMassExcluded)
+    int gone_count;
 
     __device__ __forceinline__ bool excluded(int64_t i) const {
-        const uint32_t h = static_cast<uint32_t>(i >> 3) % kExcludeBuckets;
-        if (!(buckets[h >> 5] >> (h & 31) & 1u))
-            return false;
-        for (int j = 1; j < until; j++)
-            if (par[j] == cur && tok[j] == i)
+        for (int j = 0; j < gone_count; j++)
+            if (gone[j] == i)
                 return true;
         return false;
     }
     __device__ __forceinline__ double weight(float pv, float qv) const {
-        const double w = static_cast<double>(clean_prob(pv)) - c * static_cast<double>(clean_prob(qv));
-        return w > 0.0 ? w : 0.0;
+        const double w = prob64(pv) - c * prob64(qv);
+        return __double2hiint(w) < 0 ? 0.0 : w;
     }
     __device__ __forceinline__ double at(int64_t i) const {
         const float pv = Elem<T>::from_storage(p[i]);
@@ -84,16 +83,23 @@ struct RowMass {
             return weight(pv, Elem<T>::from_storage(q[i]));
         if (mode == kMassExcluded && excluded(i))
             return 0.0;
-        return static_cast<double>(clean_prob(pv));
+        return prob64(pv);
     }
 };
 
 // Sum over [lo, hi), which a warp reads together; (p + vlo) is 16-byte aligned for the vector part [vlo, vhi).
 template <typename T>
 __device__ double warp_range_mass(const RowMass<T> &m, int64_t lo, int64_t hi, int64_t vlo, bool q_aligned) {
-    constexpr int VEC = Elem<T>::kPerVec, U = 4;
+    constexpr int VEC = Elem<T>::kPerVec, U = 16 / VEC;  // 16 elements of each row in flight a lane
     const int lane = threadIdx.x & 31;
     double s = 0.0;
+    // few ranges hold a rejected token: the others need no look at the list
+    bool look = false;
+    if (m.mode == kMassExcluded) {
+        for (int j = lane; j < m.gone_count; j += 32)
+            look |= m.gone[j] >= lo && m.gone[j] < hi;
+        look = __any_sync(kFullMask, look);
+    }
     if (lo < vlo) {  // the part in front of the first aligned vector: fewer than VEC elements
         const int64_t i = lo + lane;
         if (i < min(vlo, hi))
@@ -135,7 +141,7 @@ __device__ double warp_range_mass(const RowMass<T> &m, int64_t lo, int64_t hi, i
             } else {
 #pragma unroll
                 for (int e = 0; e < VEC; e++)
-                    s += (m.mode == kMassExcluded && m.excluded(i0 + e)) ? 0.0 : static_cast<double>(clean_prob(f[e]));
+                    s += look && m.excluded(i0 + e) ? 0.0 : prob64(f[e]);
             }
         }
     }
@@ -163,12 +169,12 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) draft_verify_kernel(const V
     float *s_chance = s_u + N;
     int *s_par = reinterpret_cast<int *>(s_chance + N);  // -1: nobody's child
     int *s_tok = s_par + N;
-    int *s_path = s_tok + N;
-    __shared__ double s_sum[2][kVerifyWarps];                       // this CTA's warp sums, by pass parity (read by the cluster)
-    __shared__ double s_all[kVerifyMaxCluster * kVerifyWarps];      // everybody's
+    int *s_path = s_tok + N, *s_gone = s_path + N;
+    __shared__ double s_all[2][kVerifyMaxCluster * kVerifyWarps];  // sums of the cluster's warps, by pass parity
     __shared__ double s_scan[kVerifyWarps];
-    __shared__ uint32_t s_buckets[kExcludeBuckets / 32];
-    __shared__ int s_last, s_found;
+    __shared__ int s_last, s_found, s_gone_count;
+
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // waited for before the first store to another CTA
 
     int used = N;
     if (a.num_nodes)
@@ -180,8 +186,8 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) draft_verify_kernel(const V
         const int64_t tok = a.index_dtype == VKOP_I64 ? static_cast<const int64_t *>(a.tokens)[b * N + i]
                                                       : static_cast<const int32_t *>(a.tokens)[b * N + i];
         const bool ok = i > 0 && i < used && par >= 0 && par < i && tok >= 0 && tok < a.vocab;
-        s_p[i] = ok ? static_cast<double>(load_prob(target + par * a.target_ns + tok)) : 0.0;
-        s_q[i] = ok && par < a.draft_rows ? static_cast<double>(load_prob(draft + par * a.draft_ns + tok)) : 1.0;
+        s_p[i] = ok ? load_prob(target + par * a.target_ns + tok) : 0.0;
+        s_q[i] = ok && par < a.draft_rows ? load_prob(draft + par * a.draft_ns + tok) : 1.0;
         s_par[i] = ok ? par : -1;
         s_tok[i] = ok ? static_cast<int>(tok) : -1;
         s_u[i] = a.u[b * N + i];
@@ -190,39 +196,81 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) draft_verify_kernel(const V
     }
     __syncthreads();
 
+    constexpr int VEC = Elem<T>::kPerVec;
+    constexpr int PER_LANE = kVerifyMaxCluster * kVerifyWarps / 32;  // ranges that a lane scans
+    const int ranges = csize * kVerifyWarps;
+    const int64_t width = ((a.vocab + ranges - 1) / ranges + VEC - 1) / VEC * VEC;
+    auto head_of = [&](const T *row) { return static_cast<int64_t>(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(T)); };
+    auto range_lo = [&](int64_t head, int r) { return r == 0 ? 0 : min(a.vocab, head + r * width); };
     int passes = 0;
-    // the sum of one pass, the same bits in every thread of the cluster; s_all keeps the sums of the ranges in row order
-    auto cluster_mass = [&](const RowMass<T> &m) {
-        constexpr int VEC = Elem<T>::kPerVec;
-        const int ranges = csize * kVerifyWarps, mine = rank * kVerifyWarps + warp;
-        const int64_t head = ((16 - (reinterpret_cast<uintptr_t>(m.p) & 15)) & 15) / sizeof(T);
-        const int64_t width = ((a.vocab + ranges - 1) / ranges + VEC - 1) / VEC * VEC;
-        const int64_t lo = mine == 0 ? 0 : min(a.vocab, head + mine * width), hi = min(a.vocab, head + (mine + 1) * width);
+    // The sum of one pass over a row, the same bits in every thread of the cluster.  Given an aim, as a share of the total:
+    // *own the range in which the prefix sum passes it, *before the prefix in front of that range.  By rounding, or for a
+    // share >= 1, none may: then the last range that holds anything.
+    auto cluster_mass = [&](const RowMass<T> &m, double share, int *own, double *before, double *aim) {
+        const int mine = rank * kVerifyWarps + warp;
+        const int64_t head = head_of(m.p);
         const bool q_aligned = (reinterpret_cast<uintptr_t>(m.q) & 15) == (reinterpret_cast<uintptr_t>(m.p) & 15);
-        const double s = warp_range_mass<T>(m, lo, hi, head, q_aligned);
-        if (lane == 0)
-            s_sum[passes & 1][warp] = s;
-        cluster.sync();
-        if (tid < ranges)
-            s_all[tid] = *cluster.map_shared_rank(&s_sum[passes & 1][tid % kVerifyWarps], tid / kVerifyWarps);
-        __syncthreads();
+        const double s = warp_range_mass<T>(m, range_lo(head, mine), min(a.vocab, head + (mine + 1) * width), head, q_aligned);
+        double *all = s_all[passes & 1];
+        if (passes == 0)
+            asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // all CTAs of the cluster run
+        if (lane < csize)
+            *cluster.map_shared_rank(&all[mine], lane) = s;
+        cluster.sync();  // (a pass apart, so that nobody still reads what the pass after the next one writes)
         passes++;
-        double t = 0.0;
-        for (int k = 0; k < ranges; k += 32) {
-            double x = k + lane < ranges ? s_all[k + lane] : 0.0;
+        double v[PER_LANE], sum = 0.0;
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1)
-                x += __shfl_xor_sync(kFullMask, x, o);
-            t += x;
+        for (int k = 0; k < PER_LANE; k++) {
+            v[k] = lane * PER_LANE + k < ranges ? all[lane * PER_LANE + k] : 0.0;
+            sum += v[k];
         }
-        return t;
+        double upto = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double y = __shfl_up_sync(kFullMask, upto, o);
+            upto += lane >= o ? y : 0.0;
+        }
+        const double total = __shfl_sync(kFullMask, upto, 31);
+        if (own) {
+            *aim = share * total;
+            double run = __shfl_up_sync(kFullMask, upto, 1);
+            run = lane == 0 ? 0.0 : run;
+            int at = -1;
+            double at_before = 0.0;
+#pragma unroll
+            for (int k = 0; k < PER_LANE; k++) {
+                if (at < 0 && run + v[k] > *aim) {
+                    at = lane * PER_LANE + k;
+                    at_before = run;
+                }
+                run += v[k];
+            }
+            unsigned hit = __ballot_sync(kFullMask, at >= 0);
+            int who = __ffs(hit) - 1;
+            if (hit == 0) {
+                run = upto - sum;
+#pragma unroll
+                for (int k = 0; k < PER_LANE; k++) {
+                    if (v[k] > 0.0) {
+                        at = lane * PER_LANE + k;
+                        at_before = run;
+                    }
+                    run += v[k];
+                }
+                hit = __ballot_sync(kFullMask, at >= 0);
+                who = 31 - __clz(hit);  // -1 for an empty row: nothing is drawn then
+            }
+            *own = __shfl_sync(kFullMask, at, who & 31);
+            *before = __shfl_sync(kFullMask, at_before, who & 31);
+        }
+        return total;
     };
 
     // ---- walk ----
     int cur = 0, last = 0, count = used > 0 ? 1 : 0;
     double c = 0.0, mass = 1.0;
     bool stale = false;  // c has grown, mass not yet taken
-    RowMass<T> m{target, draft, 0.0, kMassPlain, s_par, s_tok, s_buckets, 0, 0};
+    RowMass<T> m{target, draft, 0.0, kMassPlain, s_gone, 0};
     while (true) {
         int child = 0;
         for (int base = (last + 1) & ~31; base < used && child == 0; base += 32) {
@@ -239,7 +287,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) draft_verify_kernel(const V
             m.q = draft + cur * a.draft_ns;
             m.c = c;
             m.mode = kMassResidual;
-            mass = cluster_mass(m);
+            mass = cluster_mass(m, 0.0, nullptr, nullptr, nullptr);
             stale = false;
         }
         double left = s_p[child], scaled = mass;
@@ -282,60 +330,31 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) draft_verify_kernel(const V
         m.p = target + cur * a.target_ns;
         m.q = draft + cur * a.draft_ns;
         m.c = c;
-        m.cur = cur;
-        m.until = used;
         m.mode = kMassPlain;
         if (stale) {
             m.mode = kMassResidual;
         } else if (cur >= a.draft_rows) {  // the walk ended here: every child was tested and rejected
-            bool any = false;
+            if (tid == 0)
+                s_gone_count = 0;
+            __syncthreads();
             for (int i = tid; i < used; i += kVerifyThreads)
-                any |= s_par[i] == cur;
-            if (__syncthreads_or(any))
+                if (s_par[i] == cur)
+                    s_gone[atomicAdd(&s_gone_count, 1)] = s_tok[i];  // in any order
+            __syncthreads();
+            m.gone_count = s_gone_count;
+            if (m.gone_count > 0)
                 m.mode = kMassExcluded;
         }
-        if (m.mode == kMassExcluded) {
-            for (int i = tid; i < kExcludeBuckets / 32; i += kVerifyThreads)
-                s_buckets[i] = 0;
-            __syncthreads();
-            for (int i = tid; i < used; i += kVerifyThreads)
-                if (s_par[i] == cur) {
-                    const uint32_t h = static_cast<uint32_t>(s_tok[i] >> 3) % kExcludeBuckets;
-                    atomicOr(&s_buckets[h >> 5], 1u << (h & 31));
-                }
-            __syncthreads();
-        }
-        double total = cluster_mass(m);
+        int own = -1;
+        double before = 0.0, aim = 0.0;
+        double total = cluster_mass(m, static_cast<double>(s_u[0]), &own, &before, &aim);
         if (!(total > 0.0) && m.mode != kMassPlain) {
             m.mode = kMassPlain;  // nothing left: the distribution itself
-            total = cluster_mass(m);
+            total = cluster_mass(m, static_cast<double>(s_u[0]), &own, &before, &aim);
         }
         if (total > 0.0) {
-            const int ranges = csize * kVerifyWarps;
-            const double aim = static_cast<double>(s_u[0]) * total;
-            // the range where the prefix sum passes the aim; by rounding or a number >= 1 none may: then the last that holds anything
-            int own = -1, full = 0;
-            double before = 0.0, run = 0.0, full_before = 0.0;
-            for (int k = 0; k < ranges && own < 0; k++) {
-                if (s_all[k] > 0.0) {
-                    full = k;
-                    full_before = run;
-                }
-                if (run + s_all[k] > aim) {
-                    own = k;
-                    before = run;
-                }
-                run += s_all[k];
-            }
-            if (own < 0) {
-                own = full;
-                before = full_before;
-            }
             if (own / kVerifyWarps == rank) {
-                constexpr int VEC = Elem<T>::kPerVec;
-                const int64_t head = ((16 - (reinterpret_cast<uintptr_t>(m.p) & 15)) & 15) / sizeof(T);
-                const int64_t width = ((a.vocab + ranges - 1) / ranges + VEC - 1) / VEC * VEC;
-                const int64_t lo = own == 0 ? 0 : min(a.vocab, head + own * width), hi = min(a.vocab, head + (own + 1) * width);
+                const int64_t head = head_of(m.p), lo = range_lo(head, own), hi = min(a.vocab, head + (own + 1) * width);
                 const int64_t per = (hi - lo + kVerifyThreads - 1) / kVerifyThreads;
                 const int64_t from = min(hi, lo + tid * per), to = min(hi, from + per);
                 double sum = 0.0;
@@ -399,8 +418,6 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) draft_verify_kernel(const V
         if (tid == 0)
             a.out_count[b] = count;
     }
-    if (passes > 0)
-        cluster.sync();  // no CTA leaves while another may still read its sums
 }
 
 template <typename T>
@@ -409,7 +426,7 @@ static int launch_draft_verify_t(const vkop_draft_verify_desc &d, const VerifyAr
     int csize = 1;
     while (csize < kVerifyMaxCluster && d.batch * csize * 2 <= 2 * 148 && d.vocab / (csize * 2) >= 2048)
         csize *= 2;
-    const size_t smem = static_cast<size_t>(d.nodes) * (2 * sizeof(double) + 5 * 4);
+    const size_t smem = static_cast<size_t>(d.nodes) * (2 * sizeof(double) + 6 * 4);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(d.batch * csize));
     cfg.blockDim = dim3(kVerifyThreads);
