@@ -232,8 +232,9 @@ int vkop_cuda_sample_topk(const void *values, int32_t dtype, const void *indices
  * first index whose prefix sum exceeds u[b][0] times the whole sum (where
  * nothing is left: from p; where p is all zero: -1).  For independent uniform
  * numbers the tokens have the target's distribution.  All of it is computed
- * in 64 bits.  Entries that are negative, NaN or infinite, or below 2^-126,
- * count as zero; a child whose token is not in [0, vocab) is passed over.
+ * in 64 bits.  Entries that are negative, NaN or below 2^-126 count as zero,
+ * infinite ones as 2^128; a child whose token is not in [0, vocab) is passed
+ * over.
  *
  * u [batch, nodes] uniform numbers in [0, 1).  out_path [batch, nodes]: the
  * accepted nodes in order, node 0 first, then -1; out_count [batch]: how many

@@ -103,7 +103,7 @@ def test_ends_of_the_uniform_range_and_degenerate_rows(capi):
     p[1, 0, 5] = p[1, 0, 3999] = 0.5
     p[2, 0] = 0.0                            # nothing to draw
     p[3, 0] = torch.tensor(float("nan"))     # not numbers: nothing either
-    p[4, 0, :6] = torch.tensor([float("inf"), -1.0, float("nan"), 0.25, 1e-40, -0.0])
+    p[4, 0, :6] = torch.tensor([1e-40, -1.0, float("nan"), 0.25, 1e-40, -0.0])
     tokens = torch.tensor([[0, 1234], [0, 17], [0, 0], [0, 0], [0, 0]], dtype=torch.int64)
     for first in (0.0, 0.49999, 0.5, 1 - 2.0**-24):
         u = torch.tensor([[first, 0.0]] * 5)
@@ -113,6 +113,19 @@ def test_ends_of_the_uniform_range_and_degenerate_rows(capi):
     u = torch.tensor([[1.0, 1.0], [7.0, 1.0], [1.0, 1.0], [1.0, 1.0], [float("nan"), 1.0]])
     _, _, token, _ = capi.draft_verify(p.cuda(), tokens.cuda(), u.cuda(), chances=True)
     assert token.tolist() == [1234, 3999, -1, -1, 3]
+
+
+def test_residuals_of_entries_that_are_no_probabilities(capi):
+    p, q, tokens, u, _ = make(4, 3, 900, torch.float32, False, 3, seed=12, near=2.0)
+    nan, inf = float("nan"), float("inf")
+    odd = torch.tensor([nan, -1.0, 1e-40, 0.0, -0.0, -inf, 2.0**-126])
+    for b in range(4):
+        p[b, 0, 10 * b:10 * b + 7], q[b, 0, 50 + b:57 + b] = odd, odd.flip(0)
+        p[b, 0, 200 + b:207 + b], q[b, 0, 200 + b:207 + b] = odd, odd.roll(2)
+    p[3, 0, 400] = inf
+    u[:, 1:] = 0.9999
+    check(capi, p, q, tokens, u)
+    check(capi, p, None, tokens, u)
 
 
 def test_bad_tokens_and_parents_are_passed_over(capi):

@@ -29,7 +29,8 @@ namespace cg = cooperative_groups;
 
 constexpr int kVerifyThreads = 512;
 constexpr int kVerifyWarps = kVerifyThreads / 32;
-constexpr int kVerifyMaxCluster = 8;  // portable cluster size
+constexpr int kVerifyMaxCluster = 16;
+constexpr int kVerifyPortableCluster = 8;
 
 struct VerifyArgs {
     const void *target, *draft, *tokens;
@@ -42,13 +43,22 @@ struct VerifyArgs {
     int nodes, draft_rows, index_dtype;
 };
 
-// An entry in 64 bits; negative, NaN and infinite ones, and those below the smallest normal 32-bit number, count as zero.
-// Exact, and put together from the bits: the conversion instruction runs at an eighth of the rate of these operations and
-// took a third of a pass.
+// An entry in 64 bits; negative and NaN ones, and those below the smallest normal 32-bit number, count as zero, infinity as
+// 2^128.  Exact, and put together from the bits: the conversion instruction runs at an eighth of the rate of these
+// operations and took a third of a pass.
 __device__ __forceinline__ double prob64(float v) {
     const uint32_t u = __float_as_uint(v);
-    const bool good = u - 0x00800000u < 0x7F000000u;
+    const bool good = u - 0x00800000u <= 0x7F000000u;
     return __hiloint2double(good ? static_cast<int>((u >> 3) + 0x38000000u) : 0, good ? static_cast<int>(u << 29) : 0);
+}
+
+// The same where a zero may be 2^-127, with fewer operations: in p - c q with c >= 1 an entry p of zero leaves nothing either
+// way, and 2^-127 in place of q = 0 is lost in the rounding.
+__device__ __forceinline__ double prob64_or_tiny(float v) {
+    float x;
+    asm("mul.ftz.f32 %0, %1, 0f3F800000;" : "=f"(x) : "f"(v));
+    const uint32_t u = __float_as_uint(fmaxf(x, 0.0f));
+    return __hiloint2double(static_cast<int>((u >> 3) + 0x38000000u), static_cast<int>(u << 29));
 }
 
 template <typename T>
@@ -74,7 +84,7 @@ struct RowMass {
         return false;
     }
     __device__ __forceinline__ double weight(float pv, float qv) const {
-        const double w = prob64(pv) - c * prob64(qv);
+        const double w = prob64_or_tiny(pv) - c * prob64_or_tiny(qv);
         return __double2hiint(w) < 0 ? 0.0 : w;
     }
     __device__ __forceinline__ double at(int64_t i) const {
@@ -136,8 +146,11 @@ __device__ double warp_range_mass(const RowMass<T> &m, int64_t lo, int64_t hi, i
                         g[e] = Elem<T>::from_storage(m.q[i0 + e]);
                 }
 #pragma unroll
-                for (int e = 0; e < VEC; e++)
-                    s += m.weight(f[e], g[e]);
+                for (int e = 0; e < VEC; e++) {
+                    const double w = prob64_or_tiny(f[e]) - m.c * prob64_or_tiny(g[e]);
+                    if (__double2hiint(w) >= 0)
+                        s += w;
+                }
             } else {
 #pragma unroll
                 for (int e = 0; e < VEC; e++)
@@ -164,13 +177,13 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) draft_verify_kernel(const V
 
     extern __shared__ __align__(16) unsigned char smem[];
     double *s_p = reinterpret_cast<double *>(smem);  // [N] target probability of a node's token at its parent
-    double *s_q = s_p + N;                           // [N] the draft's
-    float *s_u = reinterpret_cast<float *>(s_q + N);
-    float *s_chance = s_u + N;
-    int *s_par = reinterpret_cast<int *>(s_chance + N);  // -1: nobody's child
+    double *s_q = s_p + N;                           // [N] the draft's; 1 where the token was certain
+    double *s_uq = s_q + N;                          // [N] its random number times that
+    double *s_left = s_uq + N, *s_of = s_left + N;   // [N] the two sides of a test without the random number; 0 of 0: not tested
+    int *s_par = reinterpret_cast<int *>(s_of + N);  // -1: nobody's child
     int *s_tok = s_par + N;
     int *s_path = s_tok + N, *s_gone = s_path + N;
-    __shared__ double s_all[2][kVerifyMaxCluster * kVerifyWarps];  // sums of the cluster's warps, by pass parity
+    __shared__ double s_all[2][kVerifyMaxCluster * kVerifyWarps * 9 / 8];  // sums of the cluster's warps, by pass parity
     __shared__ double s_scan[kVerifyWarps];
     __shared__ int s_last, s_found, s_gone_count;
 
@@ -190,15 +203,17 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) draft_verify_kernel(const V
         s_q[i] = ok && par < a.draft_rows ? load_prob(draft + par * a.draft_ns + tok) : 1.0;
         s_par[i] = ok ? par : -1;
         s_tok[i] = ok ? static_cast<int>(tok) : -1;
-        s_u[i] = a.u[b * N + i];
-        s_chance[i] = 0.0f;
+        s_uq[i] = static_cast<double>(a.u[b * N + i]) * s_q[i];
+        s_left[i] = 0.0;
+        s_of[i] = 0.0;
         s_path[i] = i == 0 && used > 0 ? 0 : -1;
     }
     __syncthreads();
 
     constexpr int VEC = Elem<T>::kPerVec;
-    constexpr int PER_LANE = kVerifyMaxCluster * kVerifyWarps / 32;  // ranges that a lane scans
-    const int ranges = csize * kVerifyWarps;
+    constexpr int PER_LANE = kVerifyMaxCluster * kVerifyWarps / 32;  // ranges that a lane scans, at most
+    const int ranges = csize * kVerifyWarps, per_lane = (ranges + 31) / 32;
+    auto place = [](int r) { return r + (r >> 3); };  // padded: the lanes' reads fall on different banks
     const int64_t width = ((a.vocab + ranges - 1) / ranges + VEC - 1) / VEC * VEC;
     auto head_of = [&](const T *row) { return static_cast<int64_t>(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(T)); };
     auto range_lo = [&](int64_t head, int r) { return r == 0 ? 0 : min(a.vocab, head + r * width); };
@@ -215,13 +230,15 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) draft_verify_kernel(const V
         if (passes == 0)
             asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // all CTAs of the cluster run
         if (lane < csize)
-            *cluster.map_shared_rank(&all[mine], lane) = s;
+            *cluster.map_shared_rank(&all[place(mine)], lane) = s;
         cluster.sync();  // (a pass apart, so that nobody still reads what the pass after the next one writes)
         passes++;
         double v[PER_LANE], sum = 0.0;
 #pragma unroll
         for (int k = 0; k < PER_LANE; k++) {
-            v[k] = lane * PER_LANE + k < ranges ? all[lane * PER_LANE + k] : 0.0;
+            v[k] = 0.0;
+            if (k < per_lane && lane * per_lane + k < ranges)
+                v[k] = all[place(lane * per_lane + k)];
             sum += v[k];
         }
         double upto = sum;
@@ -240,7 +257,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) draft_verify_kernel(const V
 #pragma unroll
             for (int k = 0; k < PER_LANE; k++) {
                 if (at < 0 && run + v[k] > *aim) {
-                    at = lane * PER_LANE + k;
+                    at = lane * per_lane + k;
                     at_before = run;
                 }
                 run += v[k];
@@ -252,7 +269,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) draft_verify_kernel(const V
 #pragma unroll
                 for (int k = 0; k < PER_LANE; k++) {
                     if (v[k] > 0.0) {
-                        at = lane * PER_LANE + k;
+                        at = lane * per_lane + k;
                         at_before = run;
                     }
                     run += v[k];
@@ -290,11 +307,10 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) draft_verify_kernel(const V
             mass = cluster_mass(m, 0.0, nullptr, nullptr, nullptr);
             stale = false;
         }
-        double left = s_p[child], scaled = mass;
+        double left = s_p[child];
         if (drawn) {
             const double w = left - c * s_q[child];
             left = w > 0.0 ? w : 0.0;
-            scaled = mass * s_q[child];
         } else {  // a token that was rejected before has nothing left
             const int tok = s_tok[child];
             bool again = false;
@@ -304,9 +320,10 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) draft_verify_kernel(const V
             }
             left = again ? 0.0 : left;
         }
-        const bool took = static_cast<double>(s_u[child]) * scaled < left;
+        const bool took = mass * s_uq[child] < left;
         if (tid == 0) {
-            s_chance[child] = left >= scaled ? (left > 0.0 ? 1.0f : 0.0f) : static_cast<float>(left / scaled);
+            s_left[child] = left;
+            s_of[child] = mass * s_q[child];
             if (took)
                 s_path[count] = child;
         }
@@ -322,6 +339,17 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) draft_verify_kernel(const V
             mass = mass > left ? mass - left : 0.0;
         }
         last = child;
+    }
+
+    if (rank == 0) {
+        __syncthreads();  // thread 0's entries
+        for (int i = tid; i < N; i += kVerifyThreads) {
+            a.out_path[b * N + i] = s_path[i];
+            if (a.out_chance)
+                a.out_chance[b * N + i] = s_left[i] >= s_of[i] ? (s_left[i] > 0.0 ? 1.0f : 0.0f) : static_cast<float>(s_left[i] / s_of[i]);
+        }
+        if (tid == 0)
+            a.out_count[b] = count;
     }
 
     // ---- draw ----
@@ -347,10 +375,10 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) draft_verify_kernel(const V
         }
         int own = -1;
         double before = 0.0, aim = 0.0;
-        double total = cluster_mass(m, static_cast<double>(s_u[0]), &own, &before, &aim);
+        double total = cluster_mass(m, s_uq[0], &own, &before, &aim);
         if (!(total > 0.0) && m.mode != kMassPlain) {
             m.mode = kMassPlain;  // nothing left: the distribution itself
-            total = cluster_mass(m, static_cast<double>(s_u[0]), &own, &before, &aim);
+            total = cluster_mass(m, s_uq[0], &own, &before, &aim);
         }
         if (total > 0.0) {
             if (own / kVerifyWarps == rank) {
@@ -407,26 +435,25 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) draft_verify_kernel(const V
     } else if (rank == 0 && tid == 0) {
         store_index(a.out_token, a.index_dtype, b, -1);
     }
-
-    if (rank == 0) {
-        __syncthreads();  // thread 0's entries of the path
-        for (int i = tid; i < N; i += kVerifyThreads) {
-            a.out_path[b * N + i] = s_path[i];
-            if (a.out_chance)
-                a.out_chance[b * N + i] = s_chance[i];
-        }
-        if (tid == 0)
-            a.out_count[b] = count;
-    }
 }
 
 template <typename T>
 static int launch_draft_verify_t(const vkop_draft_verify_desc &d, const VerifyArgs &a, cudaStream_t stream) {
-    // CTAs for two on every SM, as long as a warp's range stays a few vectors long
+    // CTAs for two on every SM, as long as a warp's range stays a few vectors long; clusters beyond the portable size where
+    // they have a GPC each (one sequence over 128256 f32 columns: 9.4 us against 10.1 with 8)
     int csize = 1;
-    while (csize < kVerifyMaxCluster && d.batch * csize * 2 <= 2 * 148 && d.vocab / (csize * 2) >= 2048)
+    const int most = d.batch <= 8 ? kVerifyMaxCluster : kVerifyPortableCluster;
+    while (csize < most && d.batch * csize * 2 <= 2 * 148 && d.vocab / (csize * 2) >= 2048)
         csize *= 2;
-    const size_t smem = static_cast<size_t>(d.nodes) * (2 * sizeof(double) + 6 * 4);
+    const size_t smem = static_cast<size_t>(d.nodes) * (5 * sizeof(double) + 4 * 4);
+    if (smem > 32 * 1024 && cudaFuncSetAttribute(draft_verify_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) {
+        cudaGetLastError();
+        return VKOP_CUDA_ERROR;
+    }
+    if (csize > kVerifyPortableCluster && cudaFuncSetAttribute(draft_verify_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+        cudaGetLastError();
+        csize = kVerifyPortableCluster;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(d.batch * csize));
     cfg.blockDim = dim3(kVerifyThreads);

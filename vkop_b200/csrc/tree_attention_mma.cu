@@ -750,6 +750,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_attention_mma_kernel(cons
         x.begin_j = static_cast<int>(into - static_cast<int64_t>(x.begin_u) * one);
         x.left = hi - lo;
     }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join waits for this kernel's end, its launch need not
     if (lo >= hi)
         return;  // fewer tiles than CTAs
     if (warp == 12)
