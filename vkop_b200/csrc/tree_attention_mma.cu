@@ -1,7 +1,7 @@
 // Attention of a tree of drafted tokens over a paged cache on the tensor cores: 16-bit types, head sizes 64 and 128.
 //
-// The rows that share a cache head (nodes x query heads a cache head) fill the M dimension of 128-row products; 64 cached
-// positions are the N dimension of S = Q K^T and the K dimension of O += P V.  Roles of a CTA (one a SM, 16 warps):
+// The rows that share a cache head (nodes x query heads a cache head) fill the M dimension of 128-row products; 64 or 128
+// cached positions are the N dimension of S = Q K^T, 64 the K dimension of O += P V.  Roles of a CTA (one a SM, 16 warps):
 //   warps 0-7    softmax: two groups of 128 threads, a thread a row.  With more than 128 rows each group has its own 128 and
 //                both see every position (ROWT = 2); otherwise one group takes the first, the other the second half of every
 //                tile of 128 positions and their sums are joined at the end (ROWT = 1).
@@ -10,11 +10,12 @@
 //                and the page size is a power of two from 8 on, tensor-map copies of up to 32 rows bring them; the others
 //                (the end of a sequence, missing pages, other page sizes) are gathered by 16-byte copies, which leave zeros
 //                where nothing is.
-//   warp 12      products, for the groups in turn (two warps that issue at the same time let the groups wait for each
-//                other's products: 1900 cycles for 64 positions of 256 rows against 1850, and 53 us against 51 for 26 rows of 64).  S (then P in its place) and O live in tensor memory; two S tiles a
-//                group alternate, so that one is being made while the other is turned into weights.  The products of a warp
+//   warp 12      products, for the groups in turn.  S (then P in its place) and O live in tensor memory.  ROWT = 1: two S
+//                tiles of 64 positions a group alternate, so that one is being made while the other is turned into weights.
+//                ROWT = 2: one S tile of 128 positions a group, the groups take turns (products 128 wide need a quarter less
+//                of the tensor pipe, which reads 128 bytes a clock of operands from shared memory).  The products of a warp
 //                are carried out in the order of their issue: the S that overwrites a P is issued behind the product that
-//                reads it, without a wait in between (with one: 2050 cycles for 64 positions).
+//                reads it, without a wait in between.
 //
 // S: exponents are taken relative to a reference that follows the row's maximum only when it grows by more than 2^8 (the sums
 // are rescaled then, in tensor memory); P is scaled by 2^kBias so that 16-bit weights stay clear of the subnormal range.
@@ -293,8 +294,7 @@ template <typename T, int D, int ROWT>
 __device__ __forceinline__ void tree_product_role(const TreeMmaArgs &g, TreeMmaExtras &x, uint32_t q_smem, uint32_t ring, int units) {
     using Shape = TreeMmaShape<D, ROWT>;
     constexpr int NB = Shape::kRing;
-    constexpr uint32_t qk = mma_instruction<T>(128, kHalf, false), pv = mma_instruction<T>(128, D, true);
-    constexpr int PER = ROWT == 2 ? 2 : 1;  // S tiles of a group in a tile of positions
+    constexpr uint32_t qk = mma_instruction<T>(128, ROWT == 2 ? kTile : kHalf, false), pv = mma_instruction<T>(128, D, true);
     volatile int *abort = &x.abort;
     const uint32_t tmem = __shfl_sync(kFullMask, x.tmem, 0);
     const uint32_t full = smem_addr(x.full), empty = smem_addr(x.empty), s_ready = smem_addr(x.s_ready), p_ready = smem_addr(x.p_ready),
@@ -318,59 +318,115 @@ __device__ __forceinline__ void tree_product_role(const TreeMmaArgs &g, TreeMmaE
     TreeWalk<Shape::kUnitCost> walk;
     walk.begin(x);
     while (walk.next(g.a, units)) {
-        const int n = (walk.j1 - walk.j0) * PER;
+        const int n = walk.j1 - walk.j0;
         wait(smem_addr(&x.q_ready), walk.seg & 1);
-        // step i of a group: O += P(i) V, then S(i + 2) in P(i)'s place; steps -2 and -1 make the first two S
-        for (int i = -2; i < n; i++) {
-            const bool weigh = i >= 0, make = i + 2 < n;
-            const bool last = ROWT == 1 || (i & 1);  // of a tile's uses: its buffers are free then
-            if (make && (ROWT == 1 || !(i & 1)))
-                wait(full + kn * 8, k_phase);
-            if (weigh && (ROWT == 1 || !(i & 1)))
-                wait(full + vn * 8, v_phase);
-            // P(i) and S(i + 2) have the same parity; tiles are counted over all units
-            const uint32_t odd = static_cast<uint32_t>(step) & 1, p_phase = static_cast<uint32_t>(step - 2) >> 1 & 1;
-#pragma unroll
-            for (int w = 0; w < 2; w++) {
-                const uint32_t half = (ROWT == 2 ? i & 1 : w) * (kHalf * 128);
-                const uint64_t qd = q_desc + (ROWT == 2 ? w * (128 * D * 2 / 16) : 0), kd = k_desc + ((kn * Shape::kBuffer + half) >> 4),
-                               vd = v_desc + ((vn * Shape::kBuffer + half) >> 4);
-                const uint32_t at = tmem + w * 2 * kHalf + odd * kHalf;
+        if constexpr (ROWT == 2) {
+            // tile i of a group: O += P V for its first half, then for its second and S(i + 1) in their place; -1 makes the first S
+            for (int i = -1; i < n; i++, step++) {
+                const bool weigh = i >= 0, make = i + 1 < n;
+                const uint32_t phase = static_cast<uint32_t>(step - 1) & 1;
+                if (make)
+                    wait(full + kn * 8, k_phase);
                 if (weigh)
-                    wait(p_ready + w * 16 + odd * 8, p_phase);
-                __syncwarp();
-                tc_fence_after();
-                if (elect_one()) {
+                    wait(full + vn * 8, v_phase);
+                const uint64_t kd = k_desc + (kn * Shape::kBuffer >> 4), vd = v_desc + (vn * Shape::kBuffer >> 4);
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    const uint32_t at = tmem + w * 2 * kHalf, to = tmem + 4 * kHalf + w * D;
                     if (weigh) {
-                        if (ok) {
+                        wait(p_ready + w * 16, phase);
+                        __syncwarp();
+                        tc_fence_after();
+                        if (elect_one() && ok) {
 #pragma unroll
                             for (int k = 0; k < kHalf / 16; k++)
-                                mma_ts(tmem + 4 * kHalf + w * D, at + k * 8, vd + k * (2048 / 16), pv, i > 0 || k > 0);
+                                mma_ts(to, at + k * 8, vd + k * (2048 / 16), pv, i > 0 || k > 0);
                         }
-                        mma_commit(pv_done + w * 16 + odd * 8);
-                        if (last && w == 1)
-                            mma_commit(empty + vn * 8);
+                        __syncwarp();
+                        wait(p_ready + w * 16 + 8, phase);
                     }
-                    if (make) {
-                        if (ok) {
+                    __syncwarp();
+                    tc_fence_after();
+                    if (elect_one()) {
+                        if (weigh) {
+                            if (ok) {
 #pragma unroll
-                            for (int k = 0; k < D / 16; k++)
-                                mma_ss(at, qd + ((k >> 2) * (128 * 128) + (k & 3) * 32) / 16, kd + ((k >> 2) * (kTile * 128) + (k & 3) * 32) / 16, qk, k > 0);
+                                for (int k = 0; k < kHalf / 16; k++)
+                                    mma_ts(to, at + kHalf + k * 8, vd + (kHalf * 128 + k * 2048) / 16, pv, true);
+                            }
+                            mma_commit(pv_done + w * 16);
+                            if (w == 1)
+                                mma_commit(empty + vn * 8);
                         }
-                        mma_commit(s_ready + w * 16 + odd * 8);
-                        if (last && w == 1)
-                            mma_commit(empty + kn * 8);
+                        if (make) {
+                            if (ok) {
+                                const uint64_t qd = q_desc + w * (128 * D * 2 / 16);
+#pragma unroll
+                                for (int k = 0; k < D / 16; k++)
+                                    mma_ss(at, qd + ((k >> 2) * (128 * 128) + (k & 3) * 32) / 16, kd + ((k >> 2) * (kTile * 128) + (k & 3) * 32) / 16, qk, k > 0);
+                            }
+                            mma_commit(s_ready + w * 16);
+                            if (w == 1)
+                                mma_commit(empty + kn * 8);
+                        }
                     }
+                    __syncwarp();
                 }
-                __syncwarp();
+                if (make)
+                    advance(kn, k_phase);
+                if (weigh)
+                    advance(vn, v_phase);
             }
-            if (make && last)
-                advance(kn, k_phase);
-            if (weigh && last)
-                advance(vn, v_phase);
-            step++;
+            step--;
+        } else {
+            // step i of a group: O += P(i) V, then S(i + 2) in P(i)'s place; steps -2 and -1 make the first two S
+            for (int i = -2; i < n; i++, step++) {
+                const bool weigh = i >= 0, make = i + 2 < n;
+                if (make)
+                    wait(full + kn * 8, k_phase);
+                if (weigh)
+                    wait(full + vn * 8, v_phase);
+                // P(i) and S(i + 2) have the same parity; tiles are counted over all units
+                const uint32_t odd = static_cast<uint32_t>(step) & 1, phase = static_cast<uint32_t>(step - 2) >> 1 & 1;
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    const uint64_t kd = k_desc + ((kn * Shape::kBuffer + w * kHalf * 128) >> 4), vd = v_desc + ((vn * Shape::kBuffer + w * kHalf * 128) >> 4);
+                    const uint32_t at = tmem + w * 2 * kHalf + odd * kHalf;
+                    if (weigh)
+                        wait(p_ready + w * 16 + odd * 8, phase);
+                    __syncwarp();
+                    tc_fence_after();
+                    if (elect_one()) {
+                        if (weigh) {
+                            if (ok) {
+#pragma unroll
+                                for (int k = 0; k < kHalf / 16; k++)
+                                    mma_ts(tmem + 4 * kHalf + w * D, at + k * 8, vd + k * (2048 / 16), pv, i > 0 || k > 0);
+                            }
+                            mma_commit(pv_done + w * 16 + odd * 8);
+                            if (w == 1)
+                                mma_commit(empty + vn * 8);
+                        }
+                        if (make) {
+                            if (ok) {
+#pragma unroll
+                                for (int k = 0; k < D / 16; k++)
+                                    mma_ss(at, q_desc + ((k >> 2) * (128 * 128) + (k & 3) * 32) / 16, kd + ((k >> 2) * (kTile * 128) + (k & 3) * 32) / 16, qk, k > 0);
+                            }
+                            mma_commit(s_ready + w * 16 + odd * 8);
+                            if (w == 1)
+                                mma_commit(empty + kn * 8);
+                        }
+                    }
+                    __syncwarp();
+                }
+                if (make)
+                    advance(kn, k_phase);
+                if (weigh)
+                    advance(vn, v_phase);
+            }
+            step -= 2;
         }
-        step -= 2;
     }
     // tensor memory may be given back once nothing writes to it any more
     if (elect_one())
@@ -396,8 +452,8 @@ __device__ __forceinline__ void tree_softmax_role(const TreeMmaArgs &g, TreeMmaE
         if (!__all_sync(kFullMask, mbar_try(smem_addr(&bar), phase & 1)))
             ok = __all_sync(kFullMask, mbar_wait(smem_addr(&bar), phase & 1, abort)) && ok;
     };
-    // a barrier serves every other product: its parity tells a phase from the one before and the one after
-    auto wait_weighed = [&](int k) { wait(x.pv_done[w][k & 1], k >> 1); };
+    // ROWT == 1: a barrier serves every other product (two may be under way): its parity tells a phase from its neighbours
+    auto wait_weighed = [&](int k) { wait(x.pv_done[w][ROWT == 2 ? 0 : k & 1], ROWT == 2 ? k : k >> 1); };
     auto row_of = [&](const TreeWalk<Shape::kUnitCost> &at) { return at.u % g.mtiles * (ROWT * 128) + (ROWT == 2 ? w * 128 : 0) + trow; };
     // queries and parents of a unit into shared memory
     auto load_unit = [&](const TreeWalk<Shape::kUnitCost> &at, bool first) {
@@ -457,72 +513,115 @@ __device__ __forceinline__ void tree_softmax_role(const TreeMmaArgs &g, TreeMmaE
         }
 
         float m_ref = -INFINITY, l = 0.0f;  // reference of the exponents in log2 units, sum of the weights
-        for (int i = 0; i < (ROWT == 2 ? 2 * n : n); i++, seen++) {
-            const int t = ROWT == 2 ? i >> 1 : i, half = ROWT == 2 ? i & 1 : w;
-            const uint32_t t_s = s_base + (seen & 1) * kHalf;
-            wait(x.s_ready[w][seen & 1], seen >> 1);
-            if (warp_live && ok) {
-                tc_fence_after();
-                uint32_t s[2][32];
-                tmem_load32(t_s, s[0]);
-                tmem_load32(t_s + 32, s[1]);
-                const int64_t t0 = static_cast<int64_t>(walk.j0 + t) * kTile + half * kHalf;
-                const uint2 there = *reinterpret_cast<const uint2 *>(&x.valid[(tile + t) & (kSlots - 1)][half * 2]);
-                tmem_wait_load();
-                tmem_settle32(s[0]);
-                tmem_settle32(s[1]);
-                if (t0 + kHalf > walk.context || (there.x & there.y) != 0xFFFFFFFFu) {
+        constexpr int HALVES = ROWT == 2 ? 2 : 1;  // of a tile that this group turns into weights
+        for (int t = 0; t < n; t++, seen++) {
+            const int odd = ROWT == 2 ? 0 : seen & 1;
+            const uint32_t t_s = s_base + odd * kHalf;
+            wait(x.s_ready[w][odd], ROWT == 2 ? seen : seen >> 1);
+            uint64_t *p_ready = ROWT == 2 ? x.p_ready[w] : &x.p_ready[w][odd];
+            if (!(warp_live && ok)) {
+                __syncwarp();
+                if ((tid & 31) == 0)
+                    for (int half = 0; half < HALVES; half++)
+                        mbar_arrive(smem_addr(&p_ready[half]));
+                continue;
+            }
+            tc_fence_after();
+            uint32_t s[2][32];  // the scores of one half at a time
+            tmem_load32(t_s, s[0]);
+            tmem_load32(t_s + 32, s[1]);
+            const int first_word = ROWT == 2 ? 0 : 2 * w;
+            const int64_t t0 = static_cast<int64_t>(walk.j0 + t) * kTile + 32 * first_word;
+            const uint32_t *there = &x.valid[(tile + t) & (kSlots - 1)][first_word];
+            uint32_t all = there[0] & there[1];
+            if (ROWT == 2)
+                all &= there[2] & there[3];
+            const bool masked = t0 + kHalf * HALVES > walk.context || all != 0xFFFFFFFFu;
+            // scores of positions c * 32 .. of the group's share that the row does not attend become -inf
+            auto mask = [&](uint32_t (&v)[32], int c) {
+                const int64_t j = t0 + 32 * c - walk.context;  // node at the first of these positions; negative: context
+                uint32_t see = 0;
+                if (j <= -32) {
+                    see = 0xFFFFFFFFu;
+                } else if (j < kTreeMaxNodes) {
+                    const int sh = static_cast<int>(j) & 31, word = static_cast<int>(j) >> 5;  // -1 .. 3
+                    uint32_t lo = 0xFFFFFFFFu, hi = 0;
 #pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        const int64_t j = t0 + 32 * c - walk.context;  // node at the first of these positions; negative: context
-                        uint32_t see = 0;
-                        if (j <= -32) {
-                            see = 0xFFFFFFFFu;
-                        } else if (j < kTreeMaxNodes) {
-                            const int sh = static_cast<int>(j) & 31, word = static_cast<int>(j) >> 5;  // -1 .. 3
-                            uint32_t lo = 0xFFFFFFFFu, hi = 0;
-#pragma unroll
-                            for (int e = 0; e < kTreeWords; e++) {
-                                lo = word == e ? anc[e] : lo;
-                                hi = word + 1 == e ? anc[e] : hi;
-                            }
-                            see = __funnelshift_r(lo, hi, sh);
-                        }
-                        see = live ? see & (c ? there.y : there.x) : 0u;
-#pragma unroll
-                        for (int e = 0; e < 32; e++)
-                            s[c][e] = see >> e & 1u ? s[c][e] : 0xFF800000u;
+                    for (int e = 0; e < kTreeWords; e++) {
+                        lo = word == e ? anc[e] : lo;
+                        hi = word + 1 == e ? anc[e] : hi;
                     }
+                    see = __funnelshift_r(lo, hi, sh);
                 }
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                see = live ? see & there[c] : 0u;
 #pragma unroll
                 for (int e = 0; e < 32; e++)
+                    v[e] = see >> e & 1u ? v[e] : 0xFF800000u;
+            };
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            auto highest = [&](const uint32_t (&v)[32]) {
 #pragma unroll
-                    for (int c = 0; c < 2; c++)
-                        top[(e & 1) * 2 + c] = fmaxf(top[(e & 1) * 2 + c], __uint_as_float(s[c][e]));
-                const float m_tile = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * g.scale;
-                if (__any_sync(kFullMask, m_tile > m_ref + kGrow)) {
-                    // (also the first tile of a unit: m_ref = -inf, nothing to rescale yet)
-                    const float m_new = fmaxf(m_ref, m_tile), keep = m_ref == m_new ? 1.0f : exp2_approx(m_ref - m_new);
-                    m_ref = m_new;
-                    l *= keep;
-                    if (i > 0) {
-                        wait_weighed(seen - 1);
-                        tc_fence_after();
+                for (int e = 0; e < 32; e++)
+                    top[e & 3] = fmaxf(top[e & 3], __uint_as_float(v[e]));
+            };
+            tmem_wait_load();
+            tmem_settle32(s[0]);
+            tmem_settle32(s[1]);
+            if (masked) {
+                mask(s[0], 0);
+                mask(s[1], 1);
+            }
+            highest(s[0]);
+            highest(s[1]);
+            if (ROWT == 2) {  // the maximum of the second half too: one reference a tile, while no product is under way
 #pragma unroll 1
-                        for (int c = 0; c < D / 32; c++) {
-                            uint32_t o[32];
-                            tmem_load32(t_o + 32 * c, o);
-                            tmem_wait_load();
-                            tmem_settle32(o);
+                for (int c = 2; c < 4; c++) {
+                    uint32_t v[32];
+                    tmem_load32(t_s + 32 * c, v);
+                    tmem_wait_load();
+                    tmem_settle32(v);
+                    if (masked)
+                        mask(v, c);
+                    highest(v);
+                }
+            }
+            const float m_tile = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * g.scale;
+            if (__any_sync(kFullMask, m_tile > m_ref + kGrow)) {
+                // (also the first tile of a unit: m_ref = -inf, nothing to rescale yet)
+                const float m_new = fmaxf(m_ref, m_tile), keep = m_ref == m_new ? 1.0f : exp2_approx(m_ref - m_new);
+                m_ref = m_new;
+                l *= keep;
+                if (t > 0) {
+                    if (ROWT == 1)
+                        wait_weighed(seen - 1);  // with one S a group it lies before this S in any case
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; c++) {
+                        uint32_t o[32];
+                        tmem_load32(t_o + 32 * c, o);
+                        tmem_wait_load();
+                        tmem_settle32(o);
 #pragma unroll
-                            for (int e = 0; e < 32; e++)
-                                o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                            tmem_store32(t_o + 32 * c, o);
-                        }
+                        for (int e = 0; e < 32; e++)
+                            o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                        tmem_store32(t_o + 32 * c, o);
                     }
                 }
-                const float off = (m_ref == -INFINITY ? 0.0f : m_ref) - kBias;
+            }
+            const float off = (m_ref == -INFINITY ? 0.0f : m_ref) - kBias;
+#pragma unroll 1
+            for (int half = 0; half < HALVES; half++) {
+                if (half > 0) {
+                    tmem_load32(t_s + kHalf, s[0]);
+                    tmem_load32(t_s + kHalf + 32, s[1]);
+                    tmem_wait_load();
+                    tmem_settle32(s[0]);
+                    tmem_settle32(s[1]);
+                    if (masked) {
+                        mask(s[0], 2);
+                        mask(s[1], 3);
+                    }
+                }
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                 uint32_t p[32];
 #pragma unroll
@@ -534,15 +633,16 @@ __device__ __forceinline__ void tree_softmax_role(const TreeMmaArgs &g, TreeMmaE
                     sum[(e & 1) * 2 + 1] += p1;
                     p[e] = TcType<T>::pack(p0, p1);
                 }
-                tmem_store32(t_s, p);
+                tmem_store32(t_s + half * kHalf, p);
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 tmem_wait_store();
+                tc_fence_before();
+                __syncwarp();
+                if ((tid & 31) == 0)
+                    mbar_arrive(smem_addr(&p_ready[half]));
             }
-            tc_fence_before();
-            __syncwarp();
-            if ((tid & 31) == 0)
-                mbar_arrive(smem_addr(&x.p_ready[w][seen & 1]));
         }
+
         // ---- the unit's rows, or this CTA's part of them ----
         // a padding node's row took part with zeros where the tile was not masked: it attends nothing
         l = live ? l : 0.0f;
@@ -566,7 +666,7 @@ __device__ __forceinline__ void tree_softmax_role(const TreeMmaArgs &g, TreeMmaE
         more = ahead.next(a, units);
         if (more)
             load_unit(ahead, false);
-        if (seen > 1)
+        if (ROWT == 1 && seen > 1)
             wait_weighed(seen - 2);
         wait_weighed(seen - 1);
         if (ROWT == 1) {  // each group reads the other's sums too
@@ -750,7 +850,6 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_attention_mma_kernel(cons
         x.begin_j = static_cast<int>(into - static_cast<int64_t>(x.begin_u) * one);
         x.left = hi - lo;
     }
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join waits for this kernel's end, its launch need not
     if (lo >= hi)
         return;  // fewer tiles than CTAs
     if (warp == 12)
