@@ -97,69 +97,63 @@ struct RowMass {
     }
 };
 
-// Sum over [lo, hi), which a warp reads together; (p + vlo) is 16-byte aligned for the vector part [vlo, vhi).
-template <typename T>
-__device__ double warp_range_mass(const RowMass<T> &m, int64_t lo, int64_t hi, int64_t vlo, bool q_aligned) {
-    constexpr int VEC = Elem<T>::kPerVec, U = 16 / VEC;  // 16 elements of each row in flight a lane
-    const int lane = threadIdx.x & 31;
-    double s = 0.0;
-    // few ranges hold a rejected token: the others need no look at the list
-    bool look = false;
-    if (m.mode == kMassExcluded) {
-        for (int j = lane; j < m.gone_count; j += 32)
-            look |= m.gone[j] >= lo && m.gone[j] < hi;
-        look = __any_sync(kFullMask, look);
-    }
-    if (lo < vlo) {  // the part in front of the first aligned vector: fewer than VEC elements
-        const int64_t i = lo + lane;
-        if (i < min(vlo, hi))
-            s += m.at(i);
-    }
-    const int64_t start = max(lo, vlo);
-    const int64_t nvec = start < hi ? (hi - start) / VEC : 0;
-    for (int64_t v = lane; v < nvec; v += 32 * U) {
-        uint4 pv[U], qv[U];
+// Vectors 32 lanes apart from v0 on, `count` in all: 16 elements of each row in flight a lane.
+template <typename T, bool RESIDUAL>
+__device__ __forceinline__ double vector_mass(const T *p, const T *q, double c, int64_t count) {
+    constexpr int VEC = Elem<T>::kPerVec, U = 16 / VEC;
+    const uint4 *pv = reinterpret_cast<const uint4 *>(p), *qv = reinterpret_cast<const uint4 *>(q);
+    double s[2] = {0.0, 0.0};
+    for (int64_t v = threadIdx.x & 31; v < count; v += 32 * U) {
+        uint4 x[U], y[U];
 #pragma unroll
-        for (int k = 0; k < U; k++)
-            if (v + 32 * k < nvec)
-                pv[k] = load_stream(reinterpret_cast<const uint4 *>(m.p + start) + v + 32 * k);
-        if (m.mode == kMassResidual && q_aligned) {
-#pragma unroll
-            for (int k = 0; k < U; k++)
-                if (v + 32 * k < nvec)
-                    qv[k] = load_stream(reinterpret_cast<const uint4 *>(m.q + start) + v + 32 * k);
+        for (int k = 0; k < U; k++) {
+            x[k] = v + 32 * k < count ? load_stream(pv + v + 32 * k) : make_uint4(0, 0, 0, 0);
+            if (RESIDUAL)
+                y[k] = v + 32 * k < count ? load_stream(qv + v + 32 * k) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int k = 0; k < U; k++) {
-            if (v + 32 * k >= nvec)
-                break;
-            const int64_t i0 = start + (v + 32 * k) * VEC;
-            float f[VEC];
-            Elem<T>::unpack(pv[k], f);
-            if (m.mode == kMassResidual) {
-                float g[VEC];
-                if (q_aligned) {
-                    Elem<T>::unpack(qv[k], g);
-                } else {
+            float f[VEC], g[VEC];
+            Elem<T>::unpack(x[k], f);
+            if (RESIDUAL)
+                Elem<T>::unpack(y[k], g);
 #pragma unroll
-                    for (int e = 0; e < VEC; e++)
-                        g[e] = Elem<T>::from_storage(m.q[i0 + e]);
-                }
-#pragma unroll
-                for (int e = 0; e < VEC; e++) {
-                    const double w = prob64_or_tiny(f[e]) - m.c * prob64_or_tiny(g[e]);
+            for (int e = 0; e < VEC; e++) {
+                if (RESIDUAL) {
+                    const double w = prob64_or_tiny(f[e]) - c * prob64_or_tiny(g[e]);
                     if (__double2hiint(w) >= 0)
-                        s += w;
+                        s[e & 1] += w;
+                } else {
+                    s[e & 1] += prob64(f[e]);
                 }
-            } else {
-#pragma unroll
-                for (int e = 0; e < VEC; e++)
-                    s += look && m.excluded(i0 + e) ? 0.0 : prob64(f[e]);
             }
         }
     }
-    const int64_t i = start + nvec * VEC + lane;  // fewer than VEC elements behind the last vector
-    if (start < hi && i < hi)
+    return s[0] + s[1];
+}
+
+// Sum over [lo, hi), which a warp reads together; p + vlo is 16-byte aligned.
+template <typename T>
+__device__ double warp_range_mass(const RowMass<T> &m, int64_t lo, int64_t hi, int64_t vlo, bool q_aligned) {
+    constexpr int VEC = Elem<T>::kPerVec;
+    const int lane = threadIdx.x & 31;
+    // few ranges hold a rejected token: only those look at the list, an element at a time; so do rows of p and q that lie
+    // differently on the 16-byte boundaries
+    bool slow = m.mode == kMassResidual && !q_aligned;
+    if (m.mode == kMassExcluded) {
+        bool look = false;
+        for (int j = lane; j < m.gone_count; j += 32)
+            look |= m.gone[j] >= lo && m.gone[j] < hi;
+        slow = __any_sync(kFullMask, look);
+    }
+    const int64_t start = max(lo, vlo);
+    const int64_t count = !slow && start < hi ? (hi - start) / VEC : 0, from = start + count * VEC;
+    double s = 0.0;
+    if (count > 0)
+        s = m.mode == kMassResidual ? vector_mass<T, true>(m.p + start, m.q + start, m.c, count) : vector_mass<T, false>(m.p + start, nullptr, 0.0, count);
+    for (int64_t i = lo + lane; i < min(start, hi); i += 32)  // in front of the first aligned vector
+        s += m.at(i);
+    for (int64_t i = from + lane; i < hi; i += 32)  // behind the last one
         s += m.at(i);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
@@ -454,21 +448,25 @@ static int launch_draft_verify_t(const vkop_draft_verify_desc &d, const VerifyAr
         cudaGetLastError();
         csize = kVerifyPortableCluster;
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(d.batch * csize));
-    cfg.blockDim = dim3(kVerifyThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(csize);
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, draft_verify_kernel<T>, a) != cudaSuccess) {
+    while (true) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(static_cast<unsigned>(d.batch * csize));
+        cfg.blockDim = dim3(kVerifyThreads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = static_cast<unsigned>(csize);
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (cudaLaunchKernelEx(&cfg, draft_verify_kernel<T>, a) == cudaSuccess)
+            break;
         cudaGetLastError();
-        return VKOP_CUDA_ERROR;
+        if (csize <= kVerifyPortableCluster)
+            return VKOP_CUDA_ERROR;
+        csize = kVerifyPortableCluster;  // no place for the larger cluster here (a part of a GPU)
     }
     note_launch();
     return VKOP_OK;
