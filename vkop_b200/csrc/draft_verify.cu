@@ -3,8 +3,8 @@
 // One thread-block cluster serves one sequence, in one launch without scratch memory.
 //
 //  walk    The probabilities that the tests compare, p(parent)[token] and q(parent)[token], do not depend on the walk:
-//          all nodes gather theirs at once.  Every warp of the cluster then walks the tree on the copies in shared memory,
-//          all with the same result, so no decision has to be handed around.  What is left of a node's distribution after
+//          all nodes gather theirs at once.  One warp of every CTA then walks the tree on the copies in shared memory, all
+//          with the same result, so no decision has to be handed between CTAs.  What is left of a node's distribution after
 //          several rejections never has to be written down: max(max(p - c q, 0) / D - q, 0) = max(p - (c + D) q, 0) / D, so
 //          one number c and the mass D describe it.
 //  mass    Only where a second child of a node is tested after a rejection, D = sum max(p - c q, 0) takes a pass over the
@@ -278,65 +278,82 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) draft_verify_kernel(const V
     };
 
     // ---- walk ----
+    __shared__ double s_c;
+    __shared__ int s_cur, s_count, s_stale, s_need;
     int cur = 0, last = 0, count = used > 0 ? 1 : 0;
     double c = 0.0, mass = 1.0;
     bool stale = false;  // c has grown, mass not yet taken
     RowMass<T> m{target, draft, 0.0, kMassPlain, s_gone, 0};
     while (true) {
-        int child = 0;
-        for (int base = (last + 1) & ~31; base < used && child == 0; base += 32) {
-            const int i = base + lane;
-            const unsigned hit = __ballot_sync(kFullMask, i > last && i < used && s_par[i] == cur);
-            if (hit)
-                child = base + __ffs(hit) - 1;
-        }
-        if (child == 0)
-            break;
-        const bool drawn = cur < a.draft_rows;
-        if (stale) {
-            m.p = target + cur * a.target_ns;
-            m.q = draft + cur * a.draft_ns;
-            m.c = c;
-            m.mode = kMassResidual;
-            mass = cluster_mass(m, 0.0, nullptr, nullptr, nullptr);
-            stale = false;
-        }
-        double left = s_p[child];
-        if (drawn) {
-            const double w = left - c * s_q[child];
-            left = w > 0.0 ? w : 0.0;
-        } else {  // a token that was rejected before has nothing left
-            const int tok = s_tok[child];
-            bool again = false;
-            for (int base = 0; base < child; base += 32) {
-                const int i = base + lane;
-                again |= __ballot_sync(kFullMask, i > 0 && i < child && s_par[i] == cur && s_tok[i] == tok) != 0;
+        if (warp == 0) {  // until it ends or a mass is needed
+            int need = 0;
+            while (true) {
+                int child = 0;
+                for (int base = (last + 1) & ~31; base < used && child == 0; base += 32) {
+                    const int i = base + lane;
+                    const unsigned hit = __ballot_sync(kFullMask, i > last && i < used && s_par[i] == cur);
+                    if (hit)
+                        child = base + __ffs(hit) - 1;
+                }
+                if (child == 0)
+                    break;
+                const bool drawn = cur < a.draft_rows;
+                if (stale) {
+                    need = 1;
+                    break;
+                }
+                double left = s_p[child];
+                if (drawn) {
+                    const double w = left - c * s_q[child];
+                    left = w > 0.0 ? w : 0.0;
+                } else {  // a token that was rejected before has nothing left
+                    const int tok = s_tok[child];
+                    bool again = false;
+                    for (int base = 0; base < child; base += 32) {
+                        const int i = base + lane;
+                        again |= __ballot_sync(kFullMask, i > 0 && i < child && s_par[i] == cur && s_tok[i] == tok) != 0;
+                    }
+                    left = again ? 0.0 : left;
+                }
+                const bool took = mass * s_uq[child] < left;
+                if (lane == 0) {
+                    s_left[child] = left;
+                    s_of[child] = mass * s_q[child];
+                    if (took)
+                        s_path[count] = child;
+                }
+                if (took) {
+                    cur = child;
+                    count++;
+                    c = 0.0;
+                    mass = 1.0;
+                } else if (drawn) {
+                    c += mass;
+                    stale = true;
+                } else {
+                    mass = mass > left ? mass - left : 0.0;
+                }
+                last = child;
             }
-            left = again ? 0.0 : left;
+            if (lane == 0)
+                s_cur = cur, s_count = count, s_stale = stale, s_need = need, s_c = c;
         }
-        const bool took = mass * s_uq[child] < left;
-        if (tid == 0) {
-            s_left[child] = left;
-            s_of[child] = mass * s_q[child];
-            if (took)
-                s_path[count] = child;
-        }
-        if (took) {
-            cur = child;
-            count++;
-            c = 0.0;
-            mass = 1.0;
-        } else if (drawn) {
-            c += mass;
-            stale = true;
-        } else {
-            mass = mass > left ? mass - left : 0.0;
-        }
-        last = child;
+        __syncthreads();
+        cur = s_cur;
+        count = s_count;
+        stale = s_stale != 0;
+        c = s_c;
+        if (!s_need)
+            break;
+        m.p = target + cur * a.target_ns;
+        m.q = draft + cur * a.draft_ns;
+        m.c = c;
+        m.mode = kMassResidual;
+        mass = cluster_mass(m, 0.0, nullptr, nullptr, nullptr);  // (ends behind a barrier: the state may be written again)
+        stale = false;
     }
 
     if (rank == 0) {
-        __syncthreads();  // thread 0's entries
         for (int i = tid; i < N; i += kVerifyThreads) {
             a.out_path[b * N + i] = s_path[i];
             if (a.out_chance)
