@@ -177,7 +177,7 @@ static TreePlan plan_parts(const vkop_tree_attention_desc &d, int rows_a_cta, in
     return p;
 }
 
-static TreePlan plan_general(const vkop_tree_attention_desc &d) { return plan_parts(d, kGenWarps, 148 * 4, 256); }
+static TreePlan plan_general(const vkop_tree_attention_desc &d) { return plan_parts(d, kGenWarps, 148 * 4, 512); }
 
 int plan_tree_attention(const vkop_tree_attention_desc &d, size_t *bytes) {
     *bytes = plan_general(d).bytes;
@@ -266,7 +266,7 @@ int launch_tree_attention(const vkop_tree_attention_desc &d, const void *q, cons
     for (int64_t s : {a.q_bs, a.q_ns, a.q_hs, a.o_bs, a.o_ns, a.o_hs, a.k_ps, a.k_ts, a.k_hs, a.v_ps, a.v_ts, a.v_hs})
         bits |= s;
     if (tree_mma_serves(d) && bits % 8 == 0)
-        return launch_tree_mma(a, d.dtype, workspace, stream);
+        return launch_tree_mma(a, d, workspace, stream);
     switch (d.dtype) {
     case VKOP_F32: return launch_t<float>(a, d, stream);
     case VKOP_F16: return launch_t<__half>(a, d, stream);

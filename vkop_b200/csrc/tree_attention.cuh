@@ -88,6 +88,6 @@ struct TreePlan {
 // tensor-core kernel (tree_attention_mma.cu): whether type and head size suit it, its scratch, the call
 bool tree_mma_serves(const vkop_tree_attention_desc &d);
 size_t tree_mma_workspace(const vkop_tree_attention_desc &d);
-int launch_tree_mma(const TreeArgs &args, int dtype, void *workspace, cudaStream_t stream);
+int launch_tree_mma(const TreeArgs &args, const vkop_tree_attention_desc &d, void *workspace, cudaStream_t stream);
 
 }  // namespace vkop_cuda

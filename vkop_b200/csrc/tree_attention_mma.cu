@@ -23,7 +23,8 @@
 // Work is cut without regard to sequence borders: all tiles of the call, sequence by sequence, head by head, are one list that
 // the CTAs share out evenly, whatever the lengths of the sequences.  A (sequence, head, rows) unit that one CTA holds entirely
 // is written out; of others every CTA leaves its part in its own two slots of the scratch memory (first and last unit of its
-// range) and the join adds them up.
+// range) and the join adds them up.  Where sequences are short, whole units are shared out instead: no scan, no
+// parts, no second launch (whole_units below).
 //
 // Bound: reading the cache once from HBM for few rows a head; around 256 rows the products and the exponentials
 // (16 a clock and SM) take as long as the copies.
@@ -47,6 +48,7 @@ struct TreeMmaArgs {
     int box_rows;     // rows of a tensor-map copy; 0: rows are gathered one by one
     int page_shift;   // log2(page_size), -1 where it is not a power of two
     int64_t *starts;  // [batch + 1] first place of a sequence in the list
+    int whole;        // whole units are shared out
     int mtiles;       // groups of ROWT * 128 rows a head
     float scale;      // |scale| * log2(e)
     uint32_t flip;    // sign bits of two elements when the scale is negative: the queries take the sign
@@ -67,7 +69,7 @@ struct TreeMmaExtras {
     uint64_t full[8], empty[8], s_ready[2][2], p_ready[2][2], pv_done[2][2], q_ready, done;
     int64_t left;
     uint32_t tmem;
-    int abort, begin_b, begin_u, begin_j, pad;
+    int abort, begin_b, begin_u, begin_j, units_left;
     alignas(16) uint32_t valid[kSlots][4];
     int bad[kSlots];
     uint8_t parents[2][kTreeMaxNodes];
@@ -85,7 +87,7 @@ __device__ __forceinline__ int tree_tiles(const TreeArgs &a, int b) {
 template <int COST>
 struct TreeWalk {
     int64_t left;  // places still to come
-    int b, u, j0, j1, tiles, seg;
+    int b, u, j0, j1, tiles, seg, units_left;
     bool first;  // the range begins inside this unit (its part goes to the CTA's first slot)
     int64_t context, length;
     int used;
@@ -94,12 +96,13 @@ struct TreeWalk {
         b = x.begin_b;
         u = x.begin_u;
         j1 = x.begin_j;
+        units_left = x.units_left;
         seg = -1;
         tiles = -1;
         first = true;
     }
     __device__ __forceinline__ bool next(const TreeArgs &a, int units) {
-        while (left > 0) {
+        while (left > 0 && units_left != 0) {
             if (tiles < 0) {
                 context = tree_context(a, b);
                 used = tree_used(a, b);
@@ -112,6 +115,7 @@ struct TreeWalk {
                 j0 = j1;
                 j1 = left < tiles - j0 ? j0 + static_cast<int>(left) : tiles;
                 left -= j1 - j0;
+                units_left--;
                 seg++;
                 return true;
             }
@@ -781,25 +785,6 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_attention_mma_kernel(cons
     const int units = a.kv_heads * g.mtiles;
     auto places = [&](int tiles) { return static_cast<int64_t>(tiles + Shape::kUnitCost) * units; };
 
-    // this CTA's range of the list of all tiles
-    int64_t *s_scan = reinterpret_cast<int64_t *>(smem);
-    const int per = (a.batch + kMmaThreads - 1) / kMmaThreads;
-    const int b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
-    int64_t sum = 0;
-    int tiles0 = 0;  // of this thread's first sequence
-    for (int b = b0; b < b1; b++) {
-        const int tiles = tree_tiles(a, b);
-        tiles0 = b == b0 ? tiles : tiles0;
-        sum += places(tiles);
-    }
-    int64_t upto = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(kFullMask, upto, o);
-        upto += lane >= o ? v : 0;
-    }
-    if (lane == 31)
-        s_scan[warp] = upto;
     if (tid == 0) {
         for (int i = 0; i < 8; i++) {
             mbar_init(smem_addr(&x.full[i]), 4);   // a copy warp each
@@ -820,38 +805,70 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_attention_mma_kernel(cons
         for (int i = 0; i < kSlots; i++)
             x.bad[i] = 0;
     }
-    __syncthreads();
-    int64_t total = 0, before = upto - sum;
-    for (int i = 0; i < kMmaThreads / 32; i++) {
-        before += i < warp ? s_scan[i] : 0;
-        total += s_scan[i];
-    }
-    const int64_t lo = blockIdx.x * total / kMmaCtas, hi = (blockIdx.x + 1) * total / kMmaCtas;
-    if (blockIdx.x == 0) {
-        int64_t at = before;
+    int64_t lo, hi;
+    if (g.whole) {  // this CTA's range of the units
+        const int64_t total = static_cast<int64_t>(a.batch) * units;
+        lo = blockIdx.x * total / kMmaCtas, hi = (blockIdx.x + 1) * total / kMmaCtas;
+        if (tid == 0) {
+            x.begin_b = static_cast<int>(lo / units);
+            x.begin_u = static_cast<int>(lo % units);
+            x.begin_j = 0;
+            x.left = 1ll << 60;
+            x.units_left = static_cast<int>(hi - lo);
+        }
+    } else {  // this CTA's range of the list of all tiles
+        int64_t *s_scan = reinterpret_cast<int64_t *>(smem);
+        const int per = (a.batch + kMmaThreads - 1) / kMmaThreads;
+        const int b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
+        int64_t sum = 0;
+        int tiles0 = 0;  // of this thread's first sequence
         for (int b = b0; b < b1; b++) {
-            g.starts[b] = at;
-            at += places(b == b0 ? tiles0 : tree_tiles(a, b));
+            const int tiles = tree_tiles(a, b);
+            tiles0 = b == b0 ? tiles : tiles0;
+            sum += places(tiles);
         }
-        if (tid == 0)
-            g.starts[a.batch] = total;
-    }
-    if (lo < hi && lo >= before && lo < before + sum) {
-        int64_t at = before;
-        int b = b0, tiles = tiles0;
-        while (lo >= at + places(tiles)) {
-            at += places(tiles);
-            tiles = tree_tiles(a, ++b);
+        int64_t upto = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t v = __shfl_up_sync(kFullMask, upto, o);
+            upto += lane >= o ? v : 0;
         }
-        x.begin_b = b;
-        const int one = tiles + Shape::kUnitCost;
-        const int64_t into = lo - at;
-        x.begin_u = into >> 32 ? static_cast<int>(into / one) : static_cast<int>(static_cast<uint32_t>(into) / static_cast<uint32_t>(one));
-        x.begin_j = static_cast<int>(into - static_cast<int64_t>(x.begin_u) * one);
-        x.left = hi - lo;
+        if (lane == 31)
+            s_scan[warp] = upto;
+        __syncthreads();
+        int64_t total = 0, before = upto - sum;
+        for (int i = 0; i < kMmaThreads / 32; i++) {
+            before += i < warp ? s_scan[i] : 0;
+            total += s_scan[i];
+        }
+        lo = blockIdx.x * total / kMmaCtas, hi = (blockIdx.x + 1) * total / kMmaCtas;
+        if (blockIdx.x == 0) {
+            int64_t at = before;
+            for (int b = b0; b < b1; b++) {
+                g.starts[b] = at;
+                at += places(b == b0 ? tiles0 : tree_tiles(a, b));
+            }
+            if (tid == 0)
+                g.starts[a.batch] = total;
+        }
+        if (lo < hi && lo >= before && lo < before + sum) {
+            int64_t at = before;
+            int b = b0, tiles = tiles0;
+            while (lo >= at + places(tiles)) {
+                at += places(tiles);
+                tiles = tree_tiles(a, ++b);
+            }
+            x.begin_b = b;
+            const int one = tiles + Shape::kUnitCost;
+            const int64_t into = lo - at;
+            x.begin_u = into >> 32 ? static_cast<int>(into / one) : static_cast<int>(static_cast<uint32_t>(into) / static_cast<uint32_t>(one));
+            x.begin_j = static_cast<int>(into - static_cast<int64_t>(x.begin_u) * one);
+            x.left = hi - lo;
+            x.units_left = 0x7FFFFFFF;
+        }
     }
     if (lo >= hi)
-        return;  // fewer tiles than CTAs
+        return;  // less work than CTAs
     if (warp == 12)
         tmem_alloc(smem_addr(&x.tmem), 512);
     tc_fence_before();
@@ -959,7 +976,20 @@ bool tree_mma_serves(const vkop_tree_attention_desc &d) {
 
 static int64_t slot_rows(const TreeArgs &a) { return a.rows > 128 ? 256 : 128; }
 
+// Whole units or an even share of all tiles?  The scan, the parts and the join cost about as much as 11 tiles, a change of
+// units as 3; whole units leave some CTAs with one more than others.  Measured, us in a graph, whole against shared (8 cache
+// heads of 128, bf16): 1 sequence of 1 / 4 / 8 tiles 9.1 / 12.5 / 17.0 against 11.9 / 15.8 / 17.6, 16 sequences of 8 tiles
+// 18.6 against 28.5, 64 sequences of 8 tiles 76 against 85.  Lengths beyond 16 tiles may differ too much within a batch.
+static bool whole_units(const vkop_tree_attention_desc &d) {
+    const int64_t longest = (d.max_context > 0 ? d.max_context : static_cast<int64_t>(d.max_pages) * d.page_size) + d.nodes;
+    const int64_t tiles = (longest + kTile - 1) / kTile, rows = static_cast<int64_t>(d.nodes) * (d.q_heads / d.kv_heads);
+    const int64_t units = d.batch * d.kv_heads * (rows > 128 ? (rows + 255) / 256 : 1);
+    return tiles <= 16 && (units + kMmaCtas - 1) / kMmaCtas * (tiles + 3) * kMmaCtas <= units * (tiles + 3) + 11 * kMmaCtas;
+}
+
 size_t tree_mma_workspace(const vkop_tree_attention_desc &d) {
+    if (whole_units(d))
+        return 0;
     const int64_t rows = static_cast<int64_t>(d.nodes) * (d.q_heads / d.kv_heads) > 128 ? 256 : 128;
     const size_t starts = (static_cast<size_t>(d.batch + 1) * 8 + 31) / 32 * 32 + 32;
     return starts + static_cast<size_t>(kMmaCtas) * 2 * rows * (d.head_dim + 2) * sizeof(float);
@@ -976,6 +1006,8 @@ static int launch_mma_t(const TreeMmaArgs &g, const CUtensorMap *maps, cudaStrea
     note_launch();
     if (check_launch() != VKOP_OK)
         return VKOP_CUDA_ERROR;
+    if (g.whole)
+        return VKOP_OK;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(g.a.batch * g.a.kv_heads * g.mtiles),
                        static_cast<unsigned>((min(g.a.rows, ROWT * 128) + kMmaJoinRows - 1) / kMmaJoinRows));
@@ -1025,9 +1057,11 @@ static bool cache_map(CUtensorMap *map, int dtype, const void *base, int64_t num
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int launch_tree_mma(const TreeArgs &args, int dtype, void *workspace, cudaStream_t stream) {
+int launch_tree_mma(const TreeArgs &args, const vkop_tree_attention_desc &d, void *workspace, cudaStream_t stream) {
+    const int dtype = d.dtype;
     TreeMmaArgs g;
     g.a = args;
+    g.whole = whole_units(d);
     workspace = reinterpret_cast<void *>((reinterpret_cast<uintptr_t>(workspace) + 31) / 32 * 32);
     g.starts = static_cast<int64_t *>(workspace);
     const size_t starts = (static_cast<size_t>(args.batch + 1) * 8 + 31) / 32 * 32;
