@@ -65,9 +65,11 @@ def test_many_rows(capi, nodes, group):
     check(capi, *case(1, nodes, 1, group, 128, 32, [400], torch.float16, False, seed=nodes))
 
 
-@pytest.mark.parametrize("page", [1, 3, 5, 16, 256])
+@pytest.mark.parametrize("page", [1, 3, 5, 8, 16, 40, 48, 96, 256, 1000])
 def test_page_sizes(capi, page):
     check(capi, *case(3, 4, 2, 2, 64, page, [0, 19, 140], torch.float16, True, seed=page))
+    check(capi, *case(2, 6, 2, 3, 128, page, [1301, 777], torch.bfloat16, True, seed=page))
+    check(capi, *case(1, 40, 1, 5, 64, page, [900], torch.bfloat16, True, seed=page))
 
 
 @pytest.mark.parametrize("dim", [64, 80])

@@ -7,10 +7,10 @@
 //                tile of 128 positions and their sums are joined at the end (ROWT = 1).
 //   warps 8-11   copies: a tile's keys and values come from their pages into a ring of buffers, in rows of 128 bytes with the
 //                128-byte swizzle that the products read.  Where 32 rows in turn are all there and belong to the context,
-//                and the page size is a power of two from 8 on, tensor-map copies of up to 32 rows bring them; the others
-//                (the end of a sequence, missing pages, other page sizes) are gathered by 16-byte copies, which leave zeros
-//                where nothing is.
-//   warp 12      products, for the groups in turn.  S (then P in its place) and O live in tensor memory.  ROWT = 1: two S
+//                and the page size is a multiple of 8, tensor-map copies of 8 to 32 rows bring them; the others (the end of
+//                a sequence, missing pages, other page sizes) are gathered by 16-byte copies, which leave zeros where
+//                nothing is.
+//   warp 14      products, for the groups in turn.  S (then P in its place) and O live in tensor memory.  ROWT = 1: two S
 //                tiles of 64 positions a group alternate, so that one is being made while the other is turned into weights.
 //                ROWT = 2: one S tile of 128 positions a group, the groups take turns (products 128 wide need a quarter less
 //                of the tensor pipe, which reads 128 bytes a clock of operands from shared memory).  The products of a warp
@@ -39,6 +39,7 @@ constexpr int kMmaThreads = 512;
 constexpr int kTile = 128;       // positions a tile: what a buffer of the ring holds
 constexpr int kHalf = 64;        // positions a product
 constexpr int kMmaCtas = 148;
+constexpr int kProductWarp = 14;  // not on the scheduler of warps 0 and 4, which have all the rows where they are few
 constexpr float kBias = 6.0f;    // log2 of the scale of the weights
 constexpr float kGrow = 8.0f;    // log2 of the growth of the maximum that is let pass; 2^(6 + 8) < 65504
 constexpr int kSlots = 8;        // tiles (and units) whose flags may be alive at once: more than a ring holds
@@ -869,7 +870,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_attention_mma_kernel(cons
     }
     if (lo >= hi)
         return;  // less work than CTAs
-    if (warp == 12)
+    if (warp == kProductWarp)
         tmem_alloc(smem_addr(&x.tmem), 512);
     tc_fence_before();
     __syncthreads();
@@ -880,12 +881,12 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_attention_mma_kernel(cons
         tree_softmax_role<T, D, ROWT>(g, x, smem, units);
     else if (warp < 12)
         tree_copy_role<T, D, ROWT>(g, &k_map, &v_map, x, ring, units);
-    else if (warp == 12)
+    else if (warp == kProductWarp)
         tree_product_role<T, D, ROWT>(g, x, q_smem, ring, units);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 12)
+    if (warp == kProductWarp)
         tmem_free(x.tmem, 512);
 }
 
@@ -1074,8 +1075,9 @@ int launch_tree_mma(const TreeArgs &args, const vkop_tree_attention_desc &d, voi
     g.page_shift = (args.page_size & (args.page_size - 1)) == 0 ? __builtin_ctz(static_cast<unsigned>(args.page_size)) : -1;
     CUtensorMap maps[2] = {};
     g.box_rows = 0;
-    if (g.page_shift >= 3 && args.max_pages > 0) {
-        const int rows = args.page_size < 32 ? args.page_size : 32;
+    // boxes of the largest power of two that divides the page size: tiles begin at multiples of it, so none crosses a page
+    const int divides = args.page_size & -args.page_size, rows = divides < 32 ? divides : 32;
+    if (rows >= 8 && args.max_pages > 0) {
         if (cache_map(&maps[0], dtype, args.k, args.num_pages, args.k_ps, args.k_ts, args.k_hs, args, rows) &&
             cache_map(&maps[1], dtype, args.v, args.num_pages, args.v_ps, args.v_ts, args.v_hs, args, rows))
             g.box_rows = rows;
