@@ -285,10 +285,12 @@ _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_get
 
 def _one_device(what: str, *tensors) -> int:
     """The index of the device that all the tensors lie on (None among them is passed over)."""
-    index = tensors[0].get_device()
+    index = tensors[0].get_device()  # -1 on the host
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.get_device() != index):
-            raise RuntimeError(f"{what}: vkop_b200 runs on CUDA device memory only, all tensors on one device")
+        if t is not None and t.get_device() != index:
+            index = -1
+    if index < 0:
+        raise RuntimeError(f"{what}: vkop_b200 runs on CUDA device memory only, all tensors on one device")
     return index
 
 

@@ -30,6 +30,8 @@
 // (16 a clock and SM) take as long as the copies.
 #include <cuda.h>
 
+#include <atomic>
+
 #include "tensor_core.cuh"
 #include "tree_attention.cuh"
 
@@ -999,9 +1001,17 @@ size_t tree_mma_workspace(const vkop_tree_attention_desc &d) {
 template <typename T, int D, int ROWT>
 static int launch_mma_t(const TreeMmaArgs &g, const CUtensorMap *maps, cudaStream_t stream) {
     constexpr int smem = TreeMmaShape<D, ROWT>::kSmem;
-    if (cudaFuncSetAttribute(tree_attention_mma_kernel<T, D, ROWT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
-        cudaGetLastError();
+    static std::atomic<uint64_t> ready{0};  // devices whose kernel has been given its shared memory
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess)
         return VKOP_CUDA_ERROR;
+    const uint64_t bit = device < 64 ? 1ull << device : 0;
+    if (!(ready.load(std::memory_order_relaxed) & bit)) {
+        if (cudaFuncSetAttribute(tree_attention_mma_kernel<T, D, ROWT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+            cudaGetLastError();
+            return VKOP_CUDA_ERROR;
+        }
+        ready.fetch_or(bit, std::memory_order_relaxed);
     }
     tree_attention_mma_kernel<T, D, ROWT><<<kMmaCtas, kMmaThreads, smem, stream>>>(g, maps[0], maps[1]);
     note_launch();
