@@ -192,6 +192,34 @@ def test_streams_and_graphs(capi):
         assert all(np.array_equal(a.cpu().numpy(), w) for a, w in zip(held, want))
 
 
+def test_calls_at_the_same_time(capi):
+    cases = [make(6, 9, 30000, torch.float32, True, 9, seed=40 + i, near=2.0) for i in range(2)]
+    want = [ref.verify(p, tokens, u, q, parents) for p, q, tokens, u, parents in cases]
+    dev = [[t.cuda() for t in c] for c in cases]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in cases], [[], []]
+    for _ in range(10):
+        for i, (st, (p, q, tokens, u, parents)) in enumerate(zip(streams, dev)):
+            with torch.cuda.stream(st):
+                got[i].append(capi.draft_verify(p, tokens, u, draft=q, parents=parents))
+    torch.cuda.synchronize()
+    assert all(np.array_equal(a.cpu().numpy(), w) for i in range(2) for g in got[i] for a, w in zip(g, want[i]))
+
+
+def test_wrapper_refusals(capi):
+    p, q, tokens, u, parents = [t.cuda() for t in make(2, 4, 50, torch.float32, True, 4, seed=44)]
+    for bad in (dict(u=u.double()), dict(u=u[:, :3]), dict(tokens=tokens.short()), dict(tokens=tokens.T.contiguous().T), dict(parents=parents.long()),
+                dict(draft=q.half()), dict(draft=q[:1]), dict(draft=q[..., :49]), dict(target=p[..., ::2]), dict(target=p[:, :1].expand(2, 4, 50)),
+                dict(num_nodes=parents[:, 0])):
+        with pytest.raises(ValueError):
+            capi.draft_verify(**(dict(target=p, tokens=tokens, u=u, draft=q, parents=parents) | bad))
+    with pytest.raises(RuntimeError):
+        capi.draft_verify(p, tokens.cpu(), u)
+    with pytest.raises(capi.VkopError) as e:  # more distributions than nodes
+        capi.draft_verify(p, tokens, u, draft=torch.cat([q, q], 1))
+    assert e.value.status == capi.INVALID_ARG
+
+
 def test_empty_batch(capi):
     path, count, token = capi.draft_verify(torch.zeros(0, 3, 10).cuda(), torch.zeros(0, 3, dtype=torch.int32).cuda(), torch.zeros(0, 3).cuda())
     assert path.shape == (0, 3) and count.shape == (0,) and token.shape == (0,)

@@ -201,6 +201,62 @@ def test_long_context_and_a_bound_that_is_too_small(capi):
     assert a[0].shape == (1, 3, 2, 64)
 
 
+@pytest.mark.parametrize("batch,nodes,kv_heads,group,dim,top", [(1500, 3, 1, 2, 64, 2500), (700, 1, 3, 1, 128, 300), (40, 70, 2, 4, 64, 4000), (3, 128, 2, 8, 128, 9000)])
+def test_many_sequences_of_every_length(capi, batch, nodes, kv_heads, group, dim, top):
+    """Long lists of tiles, several sequences a thread of the scan, several groups of rows a head: against the general kernel,
+    which takes outputs off the 16-byte boundary.  Both are off the formula by at most (2 rel + t) sum p|v| + t |o| with t half a
+    step of 16 bits and rel of 32-bit roundings (far below t here): by less than 3 t max|v| each."""
+    g = torch.Generator(device="cuda").manual_seed(batch)
+    context = (torch.rand(batch, generator=g, device="cuda") ** 2 * (top + 1)).int()
+    used = torch.randint(0, nodes + 1, (batch,), generator=g, device="cuda", dtype=torch.int32)
+    page, wide = 16, -(-(top + nodes) // 16)
+    need = (context + used + page - 1) // page
+    pool = int(need.sum()) + 3
+    order = torch.randperm(pool, generator=g, device="cuda")
+    at = torch.arange(wide, device="cuda")[None]
+    table = torch.where(at < need[:, None], order[(need.cumsum(0)[:, None] - need[:, None] + at).clamp(max=pool - 1).long()], -1).to(torch.int32)
+    k, v = (torch.empty(pool, page, kv_heads, dim, dtype=torch.float16, device="cuda").normal_(generator=g) for _ in range(2))
+    q = torch.randn(batch, nodes, kv_heads * group, dim, generator=g, device="cuda").half()
+    parents = ref.random_tree(batch, nodes, torch.Generator().manual_seed(1)).cuda()
+    args = dict(parents=parents, num_nodes=used, return_lse=True, max_context=top)
+    fast = capi.tree_attention(q, k, v, table, context, **args)
+    odd = torch.zeros(batch, nodes, kv_heads * group, dim + 1, dtype=torch.float16, device="cuda")[..., 1:]
+    slow = capi.tree_attention(q, k, v, table, context, out=odd, **args)
+    assert ((fast[0].float() - slow[0].float()).abs() <= 6 * 2.0**-11 * float(v.abs().max())).all()
+    live = torch.isfinite(slow[1])
+    assert torch.equal(live, torch.isfinite(fast[1])) and ((fast[1] - slow[1])[live].abs() <= 1e-4).all()
+
+
+def test_calls_at_the_same_time(capi):
+    """Two streams, each with scratch memory of its own."""
+    cs = [[None if t is None else t.cuda() for t in case(2, 8, 2, 4, 128, 16, lengths, torch.float16, True, seed=30 + i)] for i, lengths in enumerate(([9000, 5000], [7000, 8000]))]
+    want = [capi.tree_attention(*c[:5], parents=c[5]) for c in cs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cs]
+    got = [[], []]
+    for _ in range(10):
+        for i, (st, c) in enumerate(zip(streams, cs)):
+            with torch.cuda.stream(st):
+                got[i].append(capi.tree_attention(*c[:5], parents=c[5]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i in range(2) for o in got[i])
+
+
+def test_wrapper_refusals(capi):
+    q, k, v, table, context, parents, _ = [None if t is None else t.cuda() for t in case(2, 4, 1, 2, 64, 16, [40, 9], torch.float16, True, seed=33)]
+    for bad in (dict(context=context.long()), dict(context=context[:1]), dict(parents=parents.long()), dict(parents=parents[:, :3].contiguous()),
+                dict(num_nodes=context.float()), dict(out=torch.empty_like(q)[:, :2]), dict(out=q.float())):
+        with pytest.raises(ValueError):
+            capi.tree_attention(**(dict(q=q, k_cache=k, v_cache=v, page_table=table, context=context) | bad))
+    with pytest.raises(RuntimeError):
+        capi.tree_attention(q, k, v, table.cpu(), context)
+    with pytest.raises(capi.VkopError) as e:
+        capi.tree_attention(q, k, v, table, context, scale=float("inf"))
+    assert e.value.status == capi.INVALID_ARG
+    with pytest.raises(capi.VkopError):
+        capi.tree_attention(q.expand(2, 4, 2, 64).repeat(1, 40, 1, 1), k, v, table, context)
+
+
 def test_a_context_past_the_table(capi):
     """Lengths that the table cannot hold: the positions it has are attended, the drafted ones are out of reach."""
     for dim in (64, 80):
