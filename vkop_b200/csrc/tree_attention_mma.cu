@@ -63,7 +63,7 @@ struct TreeMmaShape {
     static constexpr int kBuffer = kTile * D * 2;
     static constexpr int kRing = D == 128 ? (ROWT == 2 ? 5 : 6) : 8;
     static constexpr int kQ = ROWT * 128 * D * 2;
-    static constexpr int kExtras = 3072;
+    static constexpr int kExtras = 3 * 1024;
     static constexpr int kUnitCost = 3;  // what a change of units costs, in tiles
     static constexpr int kSmem = kQ + kRing * kBuffer + kExtras;
 };
@@ -78,7 +78,7 @@ struct TreeMmaExtras {
     uint8_t parents[2][kTreeMaxNodes];
     float2 ml[2][128];
 };
-static_assert(sizeof(TreeMmaExtras) <= 3072, "extras");
+static_assert(sizeof(TreeMmaExtras) <= 3 * 1024, "extras");
 
 __device__ __forceinline__ int tree_tiles(const TreeArgs &a, int b) {
     const int64_t length = tree_length(a, b);
