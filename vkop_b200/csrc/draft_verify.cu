@@ -46,24 +46,27 @@ struct VerifyArgs {
 // An entry in 64 bits; negative and NaN ones, and those below the smallest normal 32-bit number, count as zero, infinity as
 // 2^128.  Exact, and put together from the bits: the conversion instruction runs at an eighth of the rate of these
 // operations and took a third of a pass.
+// (16-bit entries have no bits for the low word.)
+template <typename T>
 __device__ __forceinline__ double prob64(float v) {
     const uint32_t u = __float_as_uint(v);
     const bool good = u - 0x00800000u <= 0x7F000000u;
-    return __hiloint2double(good ? static_cast<int>((u >> 3) + 0x38000000u) : 0, good ? static_cast<int>(u << 29) : 0);
+    return __hiloint2double(good ? static_cast<int>((u >> 3) + 0x38000000u) : 0, good && sizeof(T) == 4 ? static_cast<int>(u << 29) : 0);
 }
 
 // The same where a zero may be 2^-127, with fewer operations: in p - c q with c >= 1 an entry p of zero leaves nothing either
 // way, and 2^-127 in place of q = 0 is lost in the rounding.
+template <typename T>
 __device__ __forceinline__ double prob64_or_tiny(float v) {
     float x;
     asm("mul.ftz.f32 %0, %1, 0f3F800000;" : "=f"(x) : "f"(v));
     const uint32_t u = __float_as_uint(fmaxf(x, 0.0f));
-    return __hiloint2double(static_cast<int>((u >> 3) + 0x38000000u), static_cast<int>(u << 29));
+    return __hiloint2double(static_cast<int>((u >> 3) + 0x38000000u), sizeof(T) == 4 ? static_cast<int>(u << 29) : 0);
 }
 
 template <typename T>
 __device__ __forceinline__ double load_prob(const T *p) {
-    return prob64(Elem<T>::from_storage(*p));
+    return prob64<T>(Elem<T>::from_storage(*p));
 }
 
 // What is summed over a row: p, max(p - c q, 0), or p without the rejected tokens.
@@ -84,7 +87,7 @@ struct RowMass {
         return false;
     }
     __device__ __forceinline__ double weight(float pv, float qv) const {
-        const double w = prob64_or_tiny(pv) - c * prob64_or_tiny(qv);
+        const double w = prob64_or_tiny<T>(pv) - c * prob64_or_tiny<T>(qv);
         return __double2hiint(w) < 0 ? 0.0 : w;
     }
     __device__ __forceinline__ double at(int64_t i) const {
@@ -93,7 +96,7 @@ struct RowMass {
             return weight(pv, Elem<T>::from_storage(q[i]));
         if (mode == kMassExcluded && excluded(i))
             return 0.0;
-        return prob64(pv);
+        return prob64<T>(pv);
     }
 };
 
@@ -120,11 +123,11 @@ __device__ __forceinline__ double vector_mass(const T *p, const T *q, double c, 
 #pragma unroll
             for (int e = 0; e < VEC; e++) {
                 if (RESIDUAL) {
-                    const double w = prob64_or_tiny(f[e]) - c * prob64_or_tiny(g[e]);
+                    const double w = prob64_or_tiny<T>(f[e]) - c * prob64_or_tiny<T>(g[e]);
                     if (__double2hiint(w) >= 0)
                         s[e & 1] += w;
                 } else {
-                    s[e & 1] += prob64(f[e]);
+                    s[e & 1] += prob64<T>(f[e]);
                 }
             }
         }
@@ -451,9 +454,10 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) draft_verify_kernel(const V
 template <typename T>
 static int launch_draft_verify_t(const vkop_draft_verify_desc &d, const VerifyArgs &a, cudaStream_t stream) {
     // CTAs for two on every SM, as long as a warp's range stays a few vectors long; clusters beyond the portable size where
-    // they have a GPC each (one sequence over 128256 f32 columns: 9.4 us against 10.1 with 8)
+    // the GPCs hold them all (one sequence over 128256 f32 columns: 9.4 us against 10.1 with 8, 16 trees drawn over 256000 bf16
+    // columns: 28.5 us against 34.5)
     int csize = 1;
-    const int most = d.batch <= 8 ? kVerifyMaxCluster : kVerifyPortableCluster;
+    const int most = d.batch <= 16 ? kVerifyMaxCluster : kVerifyPortableCluster;
     while (csize < most && d.batch * csize * 2 <= 2 * 148 && d.vocab / (csize * 2) >= 2048)
         csize *= 2;
     const size_t smem = static_cast<size_t>(d.nodes) * (5 * sizeof(double) + 4 * 4);
