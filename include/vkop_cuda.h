@@ -244,7 +244,7 @@ int vkop_cuda_sample_topk(const void *values, int32_t dtype, const void *indices
  * Strides are in elements, rows of the vocabulary are contiguous; 0 means
  * dense. */
 typedef struct vkop_draft_verify_desc {
-    int64_t batch;
+    int64_t batch;               /* 0 .. 2^24 */
     int64_t vocab;               /* 1 .. 2^31 - 1 */
     int64_t target_batch_stride;
     int64_t target_node_stride;
@@ -289,7 +289,7 @@ int vkop_cuda_draft_verify(const vkop_draft_verify_desc *desc, const void *targe
  * 16-byte aligned, needs no clearing and keeps nothing between calls.
  * Strides are in elements, head_dim is contiguous; 0 means dense. */
 typedef struct vkop_tree_attention_desc {
-    int64_t batch;
+    int64_t batch;               /* 0 .. 65535 */
     int64_t num_pages;
     int64_t max_context;
     int64_t q_batch_stride, q_node_stride, q_head_stride;
@@ -297,14 +297,14 @@ typedef struct vkop_tree_attention_desc {
     int64_t k_page_stride, k_token_stride, k_head_stride;
     int64_t v_page_stride, v_token_stride, v_head_stride;
     int64_t table_stride;        /* elements between rows of page_table; 0 means max_pages */
-    int32_t nodes;               /* 1 .. 128 */
-    int32_t q_heads;             /* a multiple of kv_heads */
-    int32_t kv_heads;
+    int32_t nodes;               /* 1 .. 128, nodes * q_heads <= 480000 */
+    int32_t q_heads;             /* a multiple of kv_heads, at most 256 kv_heads */
+    int32_t kv_heads;            /* 1 .. 1024 */
     int32_t head_dim;            /* a multiple of 8, at most 256 */
     int32_t page_size;           /* 1 .. 65536 */
-    int32_t max_pages;           /* columns of page_table */
+    int32_t max_pages;           /* columns of page_table; max_pages * page_size < 2^31 - 65536 */
     int32_t dtype;               /* vkop_dtype of q, the caches and out */
-    float scale;                 /* finite */
+    float scale;                 /* finite, scale * log2(e) too */
 } vkop_tree_attention_desc;
 
 int vkop_cuda_tree_attention_workspace(const vkop_tree_attention_desc *desc, size_t *bytes);
@@ -326,16 +326,16 @@ int vkop_cuda_tree_attention(const vkop_tree_attention_desc *desc, const void *q
  * position context[b] on belong to sequence b alone.  out_context does not
  * overlap context. */
 typedef struct vkop_cache_compact_desc {
-    int64_t batch;
+    int64_t batch;               /* 0 .. 2^24 */
     int64_t num_pages;
     int64_t k_layer_stride, k_page_stride, k_token_stride, k_head_stride;
     int64_t v_layer_stride, v_page_stride, v_token_stride, v_head_stride;
     int64_t table_stride;
-    int32_t layers;              /* 0 .. 65535 */
+    int32_t layers;              /* 0 .. 32767 */
     int32_t nodes;               /* columns of path, 1 .. 1024 */
-    int32_t kv_heads;
-    int32_t head_dim;
-    int32_t page_size;
+    int32_t kv_heads;            /* 1 .. 65536 */
+    int32_t head_dim;            /* 1 .. 65536; kv_heads * head_dim <= 2^30 */
+    int32_t page_size;           /* 1 .. 65536 */
     int32_t max_pages;
     int32_t dtype;
     int32_t reserved;            /* 0 */

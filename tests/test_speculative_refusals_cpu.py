@@ -127,6 +127,34 @@ def test_shapes_and_types_that_the_wrappers_refuse():
     assert capi.tree_attention_workspace_bytes(q[:1, :1, :1].expand(1, 1, 1, 64), k[:1, :, :1], k[:1, :, :1], table[:1, :1]) >= 0
 
 
+def test_a_scale_that_overflows_in_units_of_log2_is_refused():
+    """Scores are kept as scale * log2(e) * q k: 2.4e38 is finite, 2.4e38 * 1.4427 is not."""
+    need = C.c_size_t(0)
+    for scale in (2.4e38, -2.4e38):
+        assert attention(attention_desc(scale=scale)) == capi.INVALID_ARG
+        assert capi.lib().vkop_cuda_tree_attention_workspace(C.byref(attention_desc(scale=scale)), C.byref(need)) == capi.INVALID_ARG
+    assert attention(attention_desc(scale=2.3e38, batch=0)) == capi.OK
+
+
+def test_rows_too_long_to_count_are_refused():
+    """A row of all heads has at most 2^30 elements: its columns are counted in 32 bits."""
+    assert compact(compact_desc(kv_heads=65536, head_dim=65536)) == capi.UNSUPPORTED
+    assert compact(compact_desc(kv_heads=32768, head_dim=65536, batch=0), None, None, None, None, None, None, None) == capi.UNSUPPORTED
+    assert compact(compact_desc(kv_heads=16384, head_dim=65536, batch=0), None, None, None, None, None, None, None) == capi.OK
+
+
+def test_a_broadcast_workspace_is_refused(monkeypatch):
+    """Its elements are more than its memory: the length that the entry point checks would be wrong."""
+    monkeypatch.setattr(capi, "_one_device", lambda what, *tensors: 0)
+    monkeypatch.setattr(capi, "_call", lambda *a: None)
+    q, k = torch.zeros(1, 3, 4, 64, dtype=torch.float16), torch.zeros(5, 16, 2, 64, dtype=torch.float16)
+    table, context = torch.zeros(1, 4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    for bad in (torch.zeros(1, dtype=torch.uint8).expand(1 << 20), torch.zeros(1 << 20, dtype=torch.uint8)[::2], torch.zeros(1 << 20)):
+        with pytest.raises(ValueError, match="workspace"):
+            capi.tree_attention(q, k, k, table, context, workspace=bad)
+    capi.tree_attention(q, k, k, table, context, workspace=torch.zeros(1 << 20, dtype=torch.uint8))
+
+
 # ---- the 64-bit statements that the GPU tests compare with, checked against each other and by hand ----
 
 

@@ -409,6 +409,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     _whole(what, "context", context, (batch,))
     _whole(what, "parents", parents, (batch, nodes))
     _whole(what, "num_nodes", num_nodes, (batch,))
+    if workspace is not None and (workspace.dtype != torch.uint8 or not workspace.is_contiguous()):
+        raise ValueError("tree_attention: workspace is a contiguous uint8 tensor")
     if out is None:
         out = q.new_empty(q.shape)
     lse = q.new_empty((batch, nodes, heads), dtype=torch.float32) if return_lse else None
@@ -418,7 +420,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         check(L.vkop_cuda_tree_attention_workspace(ref, C.byref(need)), what)
         if need.value:
             workspace = q.new_empty(need.value, dtype=torch.uint8)
-    nbytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    nbytes = 0 if workspace is None else workspace.numel()
     _call(index, what, L.vkop_cuda_tree_attention, ref, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(),
           context.data_ptr(), _ptr(parents), _ptr(num_nodes), out.data_ptr(), _ptr(lse), _ptr(workspace), nbytes)
     return (out, lse) if return_lse else out

@@ -420,7 +420,7 @@ static int validate_tree_attention(const vkop_tree_attention_desc *desc) {
         d.max_context > 0x7FFFFFFFll - 65536 || d.nodes < 1 || d.nodes > 128 || d.kv_heads < 1 || d.kv_heads > 1024 ||
         d.q_heads < d.kv_heads || d.q_heads % d.kv_heads != 0 || d.q_heads / d.kv_heads > 256 || d.head_dim < 8 || d.head_dim > 256 ||
         d.head_dim % 8 != 0 || d.page_size < 1 || d.page_size > 65536 || d.max_pages < 0 || !float_dtype(d.dtype) ||
-        !std::isfinite(d.scale))
+        !std::isfinite(d.scale * kLog2e))
         return VKOP_INVALID_ARG;
     if (static_cast<int64_t>(d.max_pages) * d.page_size > 0x7FFFFFFFll - 65536)
         return VKOP_UNSUPPORTED;
@@ -482,6 +482,8 @@ int vkop_cuda_cache_compact(const vkop_cache_compact_desc *desc, void *k_cache, 
         d.nodes < 1 || d.nodes > 1024 || d.kv_heads < 1 || d.kv_heads > 65536 || d.head_dim < 1 || d.head_dim > 65536 ||
         d.page_size < 1 || d.page_size > 65536 || d.max_pages < 0 || !float_dtype(d.dtype) || d.reserved != 0)
         return VKOP_INVALID_ARG;
+    if (static_cast<int64_t>(d.kv_heads) * d.head_dim > 1ll << 30)
+        return VKOP_UNSUPPORTED;  // a row's columns are counted in 32 bits
     for (int64_t s : {d.k_layer_stride, d.k_page_stride, d.k_token_stride, d.k_head_stride, d.v_layer_stride, d.v_page_stride,
                       d.v_token_stride, d.v_head_stride, d.table_stride})
         if (s < 0)
